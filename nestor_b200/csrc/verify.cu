@@ -1,0 +1,211 @@
+// Verification of drafted tokens against the target's probabilities, from given random numbers.
+//
+// Sequence b has `len` drafted tokens x_0 .. x_{len-1}, drawn from the rows q_i of the draft model (or, without q, each
+// the draft's certain choice). Token i is accepted while u_i q_i(x_i) < p_i(x_i); with a accepted tokens the next token
+// is drawn from r = max(p_a - q_a, 0) after a refusal (p_a without x_a where there is no q; p_a itself where r is
+// empty) and from r = p_len otherwise: the lowest j with r_0 + .. + r_j > w (r_0 + .. + r_{V-1}). Accepted and drawn
+// tokens together are distributed as draws from p alone.
+//
+// Sums are in 64 bits: the running sum has as many steps as the vocabulary has tokens, and a sum in 32 bits would move
+// one draw in some fifty across a step. Values below 2^-126 count as zero.
+//
+// What bounds it: one or two rows of the vocabulary for each sequence, read once from HBM (a few KB are read again to
+// find the token). A row is spread over a cluster of up to 8 CTAs, which exchange their sums through distributed shared
+// memory: one launch, no workspace, a fixed order of additions.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "verify.h"
+
+namespace nbv {
+namespace cg = cooperative_groups;
+
+constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
+
+__device__ __forceinline__ float val(const float* p, long i) { return __ldg(p + i); }
+__device__ __forceinline__ float val(const __half* p, long i) { return __half2float(p[i]); }
+__device__ __forceinline__ float val(const __nv_bfloat16* p, long i) { return __bfloat162float(p[i]); }
+
+// What vocabulary entry j weighs in the draw. MODE 0: p. 1: max(p - q, 0). 2: p without entry `skip`.
+template <typename T, int MODE>
+__device__ __forceinline__ float weight(const T* p, const T* q, long skip, int j) {
+  const float x = val(p, j);
+  if constexpr (MODE == 1) {
+    const float y = val(q, j);
+    return x > y ? __fsub_rn(x, y) : 0.f;
+  }
+  if constexpr (MODE == 2) return x > 0.f && j != skip ? x : 0.f;
+  return x > 0.f ? x : 0.f;
+}
+
+// Sum of entries [a, b), lane by lane with stride 32.
+template <typename T, int MODE>
+__device__ __forceinline__ double span_sum(const T* p, const T* q, long skip, int a, int b) {
+  const int lane = threadIdx.x & 31;
+  double s = 0.;
+  int j = a + lane;
+  for (; j + 7 * 32 < b; j += 8 * 32) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = weight<T, MODE>(p, q, skip, j + 32 * i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += double(w[i]);
+  }
+  for (; j < b; j += 32) s += double(weight<T, MODE>(p, q, skip, j));
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+
+// The first entry of [a, b) at which `before` plus the running sum passes `goal`; the last one that weighs anything
+// where rounding leaves none.
+template <typename T, int MODE>
+__device__ __forceinline__ int find_entry(const T* p, const T* q, long skip, int a, int b, double before, double goal) {
+  const int lane = threadIdx.x & 31;
+  int last = -1;
+  for (int j0 = a; j0 < b; j0 += 32) {
+    const int j = j0 + lane;
+    const float w = j < b ? weight<T, MODE>(p, q, skip, j) : 0.f;
+    double s = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double up = __shfl_up_sync(0xffffffffu, s, d);
+      if (lane >= d) s += up;
+    }
+    const unsigned has = __ballot_sync(0xffffffffu, w > 0.f);
+    const unsigned hit = __ballot_sync(0xffffffffu, w > 0.f && before + s > goal);
+    if (hit) return j0 + __ffs(hit) - 1;
+    if (has) last = j0 + 31 - __clz(has);
+    before += __shfl_sync(0xffffffffu, s, 31);
+  }
+  return last;
+}
+
+// Draws from the row; returns false if nothing weighs anything. All CTAs of the cluster call it together.
+template <typename T, int MODE>
+__device__ __forceinline__ bool draw(const nb_verify_args& a, const T* p, const T* q, long skip, float w, int b, double* sums, double* all) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int CL = cluster.num_blocks(), rank = cluster.block_rank();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = a.V;
+  const int spans = CL * kWarps, per = (V + spans - 1) / spans;
+  const int mine = rank * kWarps + warp, lo = min(V, mine * per), hi = min(V, lo + per);
+  const double s = span_sum<T, MODE>(p, q, skip, lo, hi);
+  if (lane == 0) sums[warp] = s;
+  cluster.sync();
+  if (threadIdx.x < spans) all[threadIdx.x] = cluster.map_shared_rank(sums, threadIdx.x / kWarps)[threadIdx.x % kWarps];
+  __syncthreads();
+  // running sums over the spans, the same in every warp: lane by lane over 4 spans each
+  double part[4], run = 0.;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = lane * 4 + i;
+    run += at < spans ? all[at] : 0.;
+    part[i] = run;
+  }
+  double incl = run;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += up;
+  }
+  const double total = __shfl_sync(0xffffffffu, incl, 31), before = incl - run, goal = double(w) * total;
+  // the first span whose running sum passes the goal; failing that the last one that weighs anything
+  int first = 1 << 20, last = -1;
+#pragma unroll
+  for (int i = 3; i >= 0; --i) {
+    const int at = lane * 4 + i;
+    if (at < spans && all[at] > 0.) {
+      if (before + part[i] > goal) first = at;
+      last = max(last, at);
+    }
+  }
+  first = __reduce_min_sync(0xffffffffu, first);
+  last = __reduce_max_sync(0xffffffffu, last);
+  const int span = first < spans ? first : last;
+  if (span < 0) {
+    cluster.sync();      // (the sums are written again by the next draw)
+    return false;
+  }
+  if (span == mine) {
+    double ahead = 0.;
+    for (int i = 0; i < span; ++i) ahead += all[i];
+    const int j = find_entry<T, MODE>(p, q, skip, lo, hi, ahead, goal);
+    if (lane == 0) a.token[b] = j;
+  }
+  cluster.sync();        // no CTA leaves while another may read its sums
+  return true;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const nb_verify_args a) {
+  __shared__ double sums[kWarps], all[kMaxCluster * kWarps];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int b = blockIdx.x / cluster.num_blocks(), lane = threadIdx.x & 31;
+  const T* P = reinterpret_cast<const T*>(a.p) + long(b) * a.p_batch;
+  const T* Q = a.q ? reinterpret_cast<const T*>(a.q) + long(b) * a.q_batch : nullptr;
+  const int len = a.len ? min(max(a.len[b], 0), a.n) : a.n;
+  auto token = [&](int i) {
+    return a.tokens_64 ? reinterpret_cast<const long long*>(a.tokens)[long(b) * a.n + i] : (long long)(reinterpret_cast<const int*>(a.tokens)[long(b) * a.n + i]);
+  };
+  // ---- the accepted prefix (every warp for itself)
+  int accepted = len;
+  for (int i0 = 0; i0 < len; i0 += 32) {
+    const int i = i0 + lane;
+    bool ok = true;
+    if (i < len) {
+      const long long x = token(i);
+      const bool known = x >= 0 && x < a.V;
+      const float px = known ? val(P + i * a.p_row, x) : 0.f;
+      const float qx = !Q ? 1.f : (known ? val(Q + i * a.q_row, x) : 0.f);
+      ok = __fmul_rn(a.u[long(b) * a.n + i], qx) < px;
+    }
+    const unsigned refused = ~__ballot_sync(0xffffffffu, ok);
+    if (refused) {
+      accepted = i0 + __ffs(refused) - 1;
+      break;
+    }
+  }
+  // ---- the next token
+  const T* p = P + accepted * a.p_row;
+  const float w = a.w[b];
+  bool done;
+  if (accepted == len) done = draw<T, 0>(a, p, nullptr, -1, w, b, sums, all);
+  else {
+    done = Q ? draw<T, 1>(a, p, Q + accepted * a.q_row, -1, w, b, sums, all) : draw<T, 2>(a, p, nullptr, token(accepted), w, b, sums, all);
+    if (!done) done = draw<T, 0>(a, p, nullptr, -1, w, b, sums, all);
+  }
+  if (cluster.block_rank() == 0 && threadIdx.x == 0) {
+    a.accepted[b] = accepted;
+    if (!done) a.token[b] = -1;
+  }
+}
+
+}  // namespace nbv
+
+extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
+  using namespace nbv;
+  if (a->B < 0 || a->n < 0 || a->V < 1 || a->type < 0 || a->type > 2) return -1;
+  if (a->B == 0) return 0;
+  // a CTA for each 4096 entries: fewer would leave warps without work, and one CTA reads so many in a microsecond
+  int cl = 1;
+  while (cl < kMaxCluster && cl * 4096 < a->V) cl *= 2;
+  if (long(a->B) * cl > 0x7fffffffl) return -1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a->B) * cl);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cl;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t rc = a->type == 0   ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16>, *a)
+                   : a->type == 1 ? cudaLaunchKernelEx(&cfg, verify_kernel<__half>, *a)
+                                  : cudaLaunchKernelEx(&cfg, verify_kernel<float>, *a);
+  if (rc != cudaSuccess) return int(rc);
+  return int(cudaGetLastError());
+}

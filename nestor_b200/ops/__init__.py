@@ -14,6 +14,7 @@ import os
 import torch
 
 from nestor_b200.ops import reference as _ref
+from nestor_b200.ops.decode import KV8Cache, kv8_cache  # noqa: F401
 from nestor_b200.ops.reference import (  # noqa: F401  (plans + pure helpers are shared)
     ColumnPlan, DepthKeyCache, ExpertPlan, NS_COEFFS, RoutingTape, apply_rope, rope_tables, set_routing_tape,
 )
@@ -136,3 +137,9 @@ expert_bank = _dispatch("expert_bank")
 dense_swiglu = _dispatch("dense_swiglu")
 lm_head_ce = _dispatch("lm_head_ce")
 newton_schulz = _dispatch("newton_schulz")
+# incremental decoding: the 8-bit key/value cache, attention over it, verification of drafted tokens
+kv8_append = _dispatch("kv8_append")
+kv8_truncate = _dispatch("kv8_truncate")
+kv8_read = _dispatch("kv8_read")
+kv8_attention = _dispatch("kv8_attention")
+verify_draft = _dispatch("verify_draft")

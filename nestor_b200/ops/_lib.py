@@ -100,7 +100,10 @@ def check_status(device: torch.device) -> None:
     code = int(status_word(device).item())
     if code:
         status_word(device).zero_()
-        raise RuntimeError(f"nestor_b200 kernel reported status {code} (a bounded device-side wait gave up)")
+        why = "a bounded device-side wait gave up"
+        if code == 7:
+            why = "rows beyond the capacity of a key/value list, or row bounds that do not ascend: those rows were dropped"
+        raise RuntimeError(f"nestor_b200 kernel reported status {code} ({why})")
 
 
 class FlashArgs(C.Structure):

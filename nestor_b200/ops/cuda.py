@@ -23,6 +23,7 @@ from torch import Tensor
 
 from nestor_b200.ops import _lib, flash, gemm as G
 from nestor_b200.ops import reference as ref
+from nestor_b200.ops.cuda_decode import kv8_append, kv8_attention, kv8_read, kv8_truncate, verify_draft  # noqa: F401
 
 # Shapes beyond a kernel's built-in limits run the PyTorch statement of the op instead. That is never silent: the first
 # such call of each kind warns with the limit it crossed, every call is counted (``oracle_path_report()``), and

@@ -1,0 +1,160 @@
+"""Kernel bodies of the decoding ops (``csrc/kv8.cu``, ``csrc/verify.cu``); statements in :mod:`nestor_b200.ops.decode`."""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+from torch import Tensor
+
+from nestor_b200.ops import _lib
+from nestor_b200.ops import decode as D
+from nestor_b200.ops.decode import BLOCK, FLOATS, KV8Cache
+
+
+class CacheArgs(C.Structure):
+    _fields_ = [("codes", C.c_void_p * 2), ("scale", C.c_void_p * 2), ("open", C.c_void_p * 2), ("status", C.c_void_p),
+                ("L", C.c_int), ("H", C.c_int), ("nb", C.c_int), ("D", C.c_int), ("U", C.c_int), ("code", C.c_int), ("type", C.c_int)]
+
+
+class RowArgs(C.Structure):
+    _fields_ = [("src", C.c_void_p * 2), ("row_stride", C.c_long * 2), ("head_stride", C.c_long * 2), ("dst", C.c_void_p * 2),
+                ("seg", C.c_void_p), ("start", C.c_void_p), ("rows", C.c_int), ("max_rows", C.c_int)]
+
+
+class AttentionArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_row", C.c_long), ("q_head", C.c_long), ("o_row", C.c_long), ("o_head", C.c_long),
+                ("seg", C.c_void_p), ("len", C.c_void_p), ("rows", C.c_int), ("max_rows", C.c_int), ("group", C.c_int), ("q_type", C.c_int),
+                ("zero_tail", C.c_int), ("scale_log2", C.c_float)]
+
+
+class VerifyArgs(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("q", C.c_void_p), ("tokens", C.c_void_p), ("u", C.c_void_p), ("w", C.c_void_p), ("len", C.c_void_p),
+                ("accepted", C.c_void_p), ("token", C.c_void_p), ("p_batch", C.c_long), ("p_row", C.c_long), ("q_batch", C.c_long),
+                ("q_row", C.c_long), ("B", C.c_int), ("n", C.c_int), ("V", C.c_int), ("type", C.c_int), ("tokens_64", C.c_int)]
+
+
+_ready = None
+
+
+def _L():
+    global _ready
+    if _ready is None:
+        L = _lib.lib()
+        vp, p = C.c_void_p, C.POINTER
+        L.nb_kv8_append.argtypes = [p(CacheArgs), p(RowArgs), vp]
+        L.nb_kv8_truncate.argtypes = [p(CacheArgs), vp, vp]
+        L.nb_kv8_read.argtypes = [p(CacheArgs), p(RowArgs), C.c_int, vp]
+        L.nb_kv8_attention.argtypes = [p(CacheArgs), p(AttentionArgs), vp, C.c_long, vp]
+        L.nb_kv8_attention_workspace.argtypes = [C.c_int, C.c_int]
+        L.nb_verify_draft.argtypes = [p(VerifyArgs), vp]
+        for f in (L.nb_kv8_append, L.nb_kv8_truncate, L.nb_kv8_read, L.nb_kv8_attention, L.nb_verify_draft):
+            f.restype = C.c_int
+        L.nb_kv8_attention_workspace.restype = C.c_long
+        _ready = L
+    return _ready
+
+
+def _launch(fn, device: torch.device, *args, launches: int = 1) -> None:
+    """Call an entry point with the current stream of ``device`` (which need not be the current device)."""
+
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if rc != 0:
+        raise RuntimeError(f"{fn.__name__} failed with code {rc}")
+    _lib.count_launch(launches)
+
+
+def _cache_args(c: KV8Cache) -> CacheArgs:
+    a = c.__dict__.get("_args")          # (the fields are frozen: one argument block serves every call)
+    if a is None:
+        L, H, nb, U, _ = c.k_codes.shape
+        a = CacheArgs((c.k_codes.data_ptr(), c.v_codes.data_ptr()), (c.k_scale.data_ptr(), c.v_scale.data_ptr()),
+                      (c.k_open.data_ptr(), c.v_open.data_ptr()), _lib.status_word(c.device).data_ptr(), L, H, nb, c.head_dim, U,
+                      0 if c.dtype == torch.int8 else 1, FLOATS[c.k_open.dtype])
+        c.__dict__["_args"] = a
+    return a
+
+
+def _rows(t: Tensor) -> Tensor:
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def kv8_append(cache: KV8Cache, k: Tensor, v: Tensor, seg_start: Tensor, start: Tensor, max_rows: int = 1) -> None:
+    D.check_append(cache, k, v, seg_start, start, max_rows)
+    if k.shape[0] == 0:
+        return
+    k, v = _rows(k), _rows(v)
+    a = RowArgs((k.data_ptr(), v.data_ptr()), (k.stride(0), v.stride(0)), (k.stride(1), v.stride(1)), (None, None),
+                seg_start.data_ptr(), start.data_ptr(), k.shape[0], max_rows)
+    _launch(_L().nb_kv8_append, cache.device, _cache_args(cache), a)
+
+
+def kv8_truncate(cache: KV8Cache, lengths: Tensor) -> None:
+    D.check_index(lengths, cache.lists, "lengths", cache.device)
+    _launch(_L().nb_kv8_truncate, cache.device, _cache_args(cache), lengths.data_ptr())
+
+
+def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype: torch.dtype = torch.float32,
+             max_rows: int = BLOCK) -> tuple[Tensor, Tensor]:
+    D.check_read(cache, seg_start, start, rows, dtype)
+    k = torch.empty(rows, cache.heads, cache.head_dim, dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
+    if rows:
+        a = RowArgs((None, None), (0, 0), (0, 0), (k.data_ptr(), v.data_ptr()), seg_start.data_ptr(), start.data_ptr(), rows, max_rows)
+        _launch(_L().nb_kv8_read, cache.device, _cache_args(cache), a, FLOATS[dtype])
+    return k, v
+
+
+_workspace: dict[tuple[int, int, int], int] = {}
+
+
+def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor, scale: float, max_rows: int = 1,
+                  out: Tensor | None = None) -> Tensor:
+    D.check_attention(q, cache, seg_start, lengths, scale, max_rows, out)
+    given = out is not None
+    if not given:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if q.shape[0] == 0:
+        return out
+    q = _rows(q)
+    L = _L()
+    group = q.shape[1] // cache.heads
+    key = (cache.head_dim, min(max_rows * group, 32), cache.device.index)
+    size = _workspace.get(key)
+    if size is None:
+        with torch.cuda.device(cache.device):
+            size = _workspace[key] = L.nb_kv8_attention_workspace(key[0], key[1])
+    # (allocated for this call on this stream: two streams, or two captured graphs, never share it)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    a = AttentionArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), seg_start.data_ptr(),
+                      lengths.data_ptr(), q.shape[0], max_rows, group, FLOATS[q.dtype], int(not given), scale * math.log2(math.e))
+    _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, ws.data_ptr(), size, launches=2)
+    return out
+
+
+def verify_draft(target_probs: Tensor, draft_tokens: Tensor, draft_probs: Tensor | None, accept_u: Tensor, sample_u: Tensor,
+                 draft_len: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    D.check_verify(target_probs, draft_tokens, draft_probs, accept_u, sample_u, draft_len)
+    p, q = target_probs, draft_probs
+    B, n, V = p.shape[0], draft_tokens.shape[1], p.shape[2]
+    out = torch.empty(2, B, dtype=torch.int32, device=p.device)
+    if B == 0:
+        return out[0], out[1]
+    if V > 1 and p.stride(2) != 1:
+        p = p.contiguous()
+    if q is not None and V > 1 and q.stride(2) != 1:
+        q = q.contiguous()
+    if n == 0:
+        q = None
+    draft_tokens, accept_u, sample_u = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
+    a = VerifyArgs(p.data_ptr(), None if q is None else q.data_ptr(), draft_tokens.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
+                   None if draft_len is None else draft_len.data_ptr(), out.data_ptr(), out.data_ptr() + 4 * B, p.stride(0), p.stride(1),
+                   0 if q is None else q.stride(0), 0 if q is None else q.stride(1), B, n, V, FLOATS[p.dtype],
+                   int(draft_tokens.dtype == torch.int64))
+    _launch(_L().nb_verify_draft, p.device, a)
+    return out[0], out[1]

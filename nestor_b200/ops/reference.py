@@ -21,6 +21,10 @@ import torch
 import torch.nn.functional as F
 from torch import Tensor
 
+from nestor_b200.ops.decode import (  # noqa: F401  (the decoding ops' statements: 8-bit cache, draft verification)
+    kv8_append, kv8_attention, kv8_read, kv8_truncate, verify_draft,
+)
+
 # ------------------------------------------------------------------------------ plans
 
 
