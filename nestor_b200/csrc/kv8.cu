@@ -15,11 +15,14 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
+#include <algorithm>
+#include <atomic>
 #include <math.h>
 #include <type_traits>
 #include <stdint.h>
 
 #include "kv8.h"
+#include "sm100.cuh"
 
 namespace nbk {
 
@@ -264,34 +267,60 @@ __global__ void __launch_bounds__(128) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // part of a warp's work.
 //
 // Precision. q is scaled per column by a power of two into [1, 2) and rounded to fp16 (exact for bf16 and fp16
-// queries); probabilities are multiplied by 2^14 before their rounding to fp16, so that weights down to 2^-28 keep 11
-// bits, and the sum of the softmax adds the rounded weights. With SPLIT (fp32 queries) both are
-// split into two fp16 numbers, which keeps 22 bits.
+// queries, two fp16 numbers for fp32 ones); probabilities are multiplied by 2^7 before their rounding to fp16, so that
+// weights down to 2^-21 of the largest keep 11 bits, and the sum of the softmax adds the rounded weights. Where the
+// output has more than bf16's 8 bits, probabilities are two fp16 numbers as well, which keeps 22.
 //
-// Division of work. All blocks of all (list, head, column tile) tasks form one line that is cut into equal pieces, one
-// for each warp of the grid: no tail, whatever the lengths, and no host knowledge of them. A warp that owns a whole
-// task writes its output; pieces of a task that is cut go to a workspace and `attn_join` adds them in order, so results
-// do not depend on the schedule.
-constexpr float kShift = 14.f;       // log2 of the factor on the probabilities
-constexpr int kWarps = 4;
-constexpr int kMaxLists = 4096;      // lists in one launch (their prefix sums stay in shared memory)
+// Division of work. All blocks of all (list, head, column tile) tasks form one line that is cut into units, whatever the
+// lengths and without the host knowing them. A warp that owns a whole task writes its output; pieces of a task that is
+// cut go to a workspace and `attn_join` adds them in order, so results do not depend on the schedule. Short lines: one
+// unit a warp. Long ones (32 blocks a warp and more): two thirds in one unit a warp, the rest in three times as many that
+// the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: 88 to 128 us).
+constexpr float kShift = 7.f;        // log2 of the factor on the probabilities
+constexpr float kSlack = 8.f;        // how far (log2) a score may pass the running maximum; 2^(kShift + kSlack) fits fp16
+constexpr int kJoin = 4;             // warps of a CTA of attn_join
+constexpr int kMaxLists = 1024;      // lists in one launch (their prefix sums stay in shared memory)
 
 struct Attn {
   nb_kv8_cache c;
   nb_kv8_attn a;
-  float* ws;
+  float* ws;          // pieces: slot 2u for a task that unit u continues, 2u + 1 for one that it begins
   long* cum;
-  int workers, min_blocks;
+  int* next;          // units handed out beyond the first `workers`
+  int workers, dynamic;
 };
 
-__device__ __forceinline__ uint4 ld_stream(const uint4* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
+constexpr int kShares = 3;           // small units for each warp of a long line
+constexpr int kLong = 32;            // blocks a warp from which on a line is long (a small unit has 3 blocks then)
+struct Cuts {
+  long total, head;                  // blocks; those in the first `workers` units
+  int workers, units;
+  __device__ __forceinline__ Cuts(const Attn& k, long t) : total(t) {
+    if (k.dynamic && t >= long(kLong) * k.workers) {
+      workers = k.workers;
+      units = (1 + kShares) * workers;
+      head = t - t / 3;
+    } else {
+      units = workers = int(max(1l, min(long(k.workers), t)));
+      head = t;
+    }
+  }
+  __device__ __forceinline__ long begin(int u) const {
+    return u <= workers ? u * head / workers : head + (u - workers) * (total - head) / (units - workers);
+  }
+  __device__ __forceinline__ int of(long pos) const {
+    return pos < head ? int(((pos + 1) * workers - 1) / head) : workers + int(((pos - head + 1) * (units - workers) - 1) / (total - head));
+  }
+};
+
 __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// d = a b + (c0, c1, c0, c1): the first product of a chain, with what a column's sums begin at
+__device__ __forceinline__ void mma_from(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1, float c0, float c1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned y;
@@ -309,11 +338,17 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// Four codes -> two half2 (bytes 0, 1 and bytes 2, 3). int8: the byte with its sign bit flipped is 128 + x; in the low
-// bits of an fp16 with the exponent of 1024 it reads 1152 + x, and the subtraction is exact. e4m3 is a subset of fp16.
-template <int CODE>
+// Four codes -> two half2 (bytes 0, 1 and bytes 2, 3). e4m3 is a subset of fp16. An int8 with its sign bit flipped is
+// u = 128 + x. RAW: the byte alone, the fp16 subnormal u 2^-24; the products' sums carry 128 sum(q), which the caller
+// takes off (3 instructions for 4 codes). Otherwise the byte in the low bits of an fp16 with the exponent of 1024 reads
+// 1152 + x, and the subtraction is exact (5 instructions, for results that keep more than 16 bits).
+template <int CODE, bool RAW>
 __device__ __forceinline__ void widen(unsigned w, unsigned& lo, unsigned& hi) {
-  if constexpr (CODE == 0) {
+  if constexpr (CODE == 0 && RAW) {
+    const unsigned x = w ^ 0x80808080u;
+    lo = __byte_perm(x, 0u, 0x4140);
+    hi = __byte_perm(x, 0u, 0x4342);
+  } else if constexpr (CODE == 0) {
     const unsigned x = w ^ 0x80808080u;
     const __half2 bias = __floats2half2_rn(1152.f, 1152.f);
     unsigned a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
@@ -328,11 +363,14 @@ __device__ __forceinline__ void widen(unsigned w, unsigned& lo, unsigned& hi) {
   }
 }
 
-__device__ __forceinline__ float load_any(const void* base, long i, int type) {
-  if (type == 2) return reinterpret_cast<const float*>(base)[i];
-  if (type == 1) return __half2float(reinterpret_cast<const __half*>(base)[i]);
-  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(base)[i]);
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
 }
+
 __device__ __forceinline__ void store_any(void* base, long i, int type, float x) {
   if (type == 2) reinterpret_cast<float*>(base)[i] = x;
   else if (type == 1) reinterpret_cast<__half*>(base)[i] = __float2half_rn(x);
@@ -341,36 +379,95 @@ __device__ __forceinline__ void store_any(void* base, long i, int type, float x)
 
 // What a list brings to a launch: rows n from s0 on, entries len, blocks nb, column tiles.
 struct ListWork { int s0, n, len, nb, tiles; };
-__device__ __forceinline__ ListWork list_work(const Attn& k, int l, int columns) {
+__device__ __forceinline__ ListWork sized(int s0, int n, int len, int group, int columns) {
   ListWork w;
-  w.s0 = k.a.seg[l];
-  const int s1 = k.a.seg[l + 1], cap = k.c.nb * kBlock, len = k.a.len[l];
-  w.n = w.s0 >= 0 && s1 <= min(k.a.rows, k.a.seg[k.c.L]) ? max(0, s1 - w.s0) : 0;
-  w.len = min(max(len, 0), cap);
-  w.nb = max(1, (w.len + kBlock - 1) / kBlock);
-  w.tiles = (w.n * k.a.group + columns - 1) / columns;
+  w.s0 = s0;
+  w.n = n;
+  w.len = len;
+  w.nb = max(1, (len + kBlock - 1) / kBlock);
+  w.tiles = (n * group + columns - 1) / columns;
   return w;
 }
-
-__device__ __forceinline__ int pieces(long total, int workers, int min_blocks) {
-  return int(max(1l, min(long(workers), (total + min_blocks - 1) / min_blocks)));
+__device__ __forceinline__ ListWork list_work(const Attn& k, int l, int end, int columns) {      // end = seg[L]
+  const int s0 = k.a.seg[l], s1 = k.a.seg[l + 1], len = k.a.len[l];
+  return sized(s0, s0 >= 0 && s1 <= min(k.a.rows, end) ? max(0, s1 - s0) : 0, min(max(len, 0), k.c.nb * kBlock), k.a.group, columns);
 }
 
-template <int UMAX, int NT, int CODE, bool SPLIT>
-__global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
-  constexpr int PAIRS = (UMAX + 1) / 2, COLS = 8 * NT, SP = SPLIT ? 2 : 1;
-  extern __shared__ long cum[];                 // [L + 1] blocks of all tasks before list l
-  __shared__ long part[kWarps];
+__device__ __forceinline__ float tile_max(const float (&s)[4][4], int i) {
+  return fmaxf(fmaxf(fmaxf(s[0][i], s[0][2 + i]), fmaxf(s[1][i], s[1][2 + i])), fmaxf(fmaxf(s[2][i], s[2][2 + i]), fmaxf(s[3][i], s[3][2 + i])));
+}
+
+// One CTA an SM, as many warps as its registers carry. Shared memory of one warp: a ring filled by bulk copies that the
+// warp itself issues. Nothing is shared between warps after the prologue, so there is no barrier but the copies' own.
+// Narrow heads: two stages of a block (keys and values together, one wait a block). Wide heads: three stages of half a
+// block, which leaves room for more warps. 16 x 10 KB, 16 x 12 KB, 12 x 15 KB or 8 x 24 KB.
+__host__ __device__ constexpr int halves_of(int umax) { return umax <= 5 ? 2 : 1; }
+__host__ __device__ constexpr int stages_of(int umax) { return umax <= 5 ? 2 : 3; }
+__host__ __device__ constexpr int warps_of(int umax, int nt) { return nt > 1 ? (umax <= 5 ? 12 : 8) : umax <= 8 ? 16 : umax <= 10 ? 12 : 8; }
+
+__device__ __forceinline__ uint4 lds(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+
+// A place in the line of blocks: list, head, column tile, block and the blocks from here on that follow in one run.
+struct Run {
+  int l, h, tile, b, blocks;
+  ListWork w;
+};
+__device__ __forceinline__ Run run_at(const Attn& k, const long* cum, const int* lists, long pos, long end, int columns) {
+  int lo = 0, hi = k.c.L;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cum[mid] <= pos) lo = mid; else hi = mid;
+  }
+  const ListWork w = sized(lists[3 * lo], lists[3 * lo + 1], lists[3 * lo + 2], k.a.group, columns);
+  const int in_list = int(pos - cum[lo]), task = in_list / w.nb;
+  Run r;
+  r.l = lo;
+  r.b = in_list - task * w.nb;
+  r.h = task / w.tiles;
+  r.tile = task - r.h * w.tiles;
+  r.blocks = int(min(long(w.nb - r.b), end - pos));
+  r.w = w;
+  return r;
+}
+
+template <int UMAX, int NT, int CODE, typename T>
+__global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const Attn k) {
+  constexpr int PAIRS = (UMAX + 1) / 2, COLS = 8 * NT, STAGES = stages_of(UMAX), HALVES = halves_of(UMAX), WARPS = warps_of(UMAX, NT);
+  // fp16 numbers that a query element and a probability are held in
+  constexpr int QS = sizeof(T) == 4 ? 2 : 1, PS = std::is_same_v<T, __nv_bfloat16> ? 1 : 2;
+  // int8 codes enter the products as (128 + x) 2^-24, queries as [2^14, 2^15)
+  constexpr bool RAW = QS == 1, BIASED = RAW && CODE == 0;
+  constexpr float kUnit = BIASED ? 0x1p24f : 1.f;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long part[WARPS];
+  __shared__ uint64_t bars[WARPS][STAGES];
   const int L = k.c.L, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int U = k.c.U, D = k.c.D;
+  const uint32_t half = U * 512;
+  const uint32_t stage = half * HALVES;
+  uint8_t* ring = smem + warp * STAGES * stage;
+  long* cum = reinterpret_cast<long*>(smem + WARPS * STAGES * stage);      // [L + 1] blocks of all tasks before list l
+  int* lists = reinterpret_cast<int*>(cum + L + 1);                         // [L][3] first row, rows, entries
+  asm volatile("griddepcontrol.launch_dependents;");      // (attn_join waits for this grid before it reads what it wrote)
 
   // ---- prefix sums of the lists' work
-  for (int l = threadIdx.x; l < L; l += blockDim.x) {
-    const ListWork w = list_work(k, l, COLS);
+  const int seg_end = k.a.seg[L];
+#pragma unroll 4
+  for (int l = threadIdx.x; l < L; l += WARPS * 32) {
+    const ListWork w = list_work(k, l, seg_end, COLS);
     cum[l + 1] = w.n ? k.c.H * w.tiles * w.nb : 0;
-    if (blockIdx.x == 0 && (k.a.len[l] > k.c.nb * kBlock || k.a.seg[l + 1] > min(k.a.rows, k.a.seg[L]) || k.a.seg[l] < 0 || k.a.seg[l + 1] < k.a.seg[l]))
+    lists[3 * l] = w.s0;
+    lists[3 * l + 1] = w.n;
+    lists[3 * l + 2] = w.len;
+    if (blockIdx.x == 0 && (k.a.len[l] > k.c.nb * kBlock || k.a.seg[l + 1] > min(k.a.rows, seg_end) || k.a.seg[l] < 0 || k.a.seg[l + 1] < k.a.seg[l]))
       atomicCAS(k.c.status, 0, kStatusRange);
   }
+  if (lane < STAGES) nb::mbar_init(&bars[warp][lane], 1);
+  nb::fence_barrier_init();
   __syncthreads();
   const int each = (L + blockDim.x - 1) / blockDim.x, l0 = min(L, int(threadIdx.x) * each), l1 = min(L, l0 + each);
   long sum = 0;
@@ -395,39 +492,108 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
     for (int l = threadIdx.x; l <= L; l += blockDim.x) k.cum[l] = cum[l];
   const long total = cum[L];
   if (total == 0) return;
-  const int P = pieces(total, k.workers, k.min_blocks);
-  const int worker = warp * gridDim.x + blockIdx.x;
-  if (worker >= P) return;
-  long pos = worker * total / P;
-  const long pos_end = (worker + 1) * total / P;
+  const Cuts cuts(k, total);
+  int unit = warp * gridDim.x + blockIdx.x;
+  if (unit >= cuts.workers) return;
 
-  while (pos < pos_end) {
-    // ---- which task
-    int lo = 0, hi = L;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cum[mid] <= pos) lo = mid; else hi = mid;
+  // ---- the copies, over run and unit borders, STAGES ahead: keys of a block and its values (in one stage or in two), the
+  // next block, ... A unit that the copies fetch is `unit_next` until the arithmetic gets there (units are longer than the
+  // ring, so there is never more than one).
+  long feed_pos = cuts.begin(unit), feed_end = cuts.begin(unit + 1), feed_at = 0;
+  int feed_left = 0, feed_slot = 0, unit_next = -1;
+  bool feed_values = false, more = cuts.units > cuts.workers;
+  auto feed = [&]() {
+    if (feed_left == 0) {
+      if (feed_pos >= feed_end) {
+        if (!more) return;
+        int u = 0;
+        if (lane == 0) u = cuts.workers + atomicAdd(k.next, 1);
+        u = __shfl_sync(0xffffffffu, u, 0);
+        more = u < cuts.units;
+        if (!more) return;
+        unit_next = u;
+        feed_pos = cuts.begin(u);
+        feed_end = cuts.begin(u + 1);
+      }
+      const Run r = run_at(k, cum, lists, feed_pos, feed_end, COLS);
+      feed_at = ((long(r.l) * k.c.H + r.h) * k.c.nb + r.b) * long(half);
+      feed_left = r.blocks;
+      feed_pos += r.blocks;
     }
-    const int l = lo;
-    const ListWork w = list_work(k, l, COLS);
-    const int in_list = int(pos - cum[l]), task = in_list / w.nb, b0 = in_list - task * w.nb;
-    const int h = task / w.tiles, tile = task - h * w.tiles;
-    const int b1 = int(min(long(w.nb), b0 + (pos_end - pos)));
-    pos += b1 - b0;
-    const long lh = long(l) * k.c.H + h;
-    const uint4* kp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(k.c.codes[0]) + lh * k.c.nb * (long(U) * 512)) + lane;
-    const uint4* vp = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(k.c.codes[1]) + lh * k.c.nb * (long(U) * 512)) + lane;
+    if (lane == 0) {
+      uint64_t* bar = &bars[warp][feed_slot];
+      uint8_t* to = ring + feed_slot * stage;
+      nb::mbar_expect_tx(bar, stage);
+      if (HALVES == 2) {
+        nb::bulk_load(to, reinterpret_cast<const uint8_t*>(k.c.codes[0]) + feed_at, half, bar);
+        nb::bulk_load(to + half, reinterpret_cast<const uint8_t*>(k.c.codes[1]) + feed_at, half, bar);
+      } else {
+        nb::bulk_load(to, reinterpret_cast<const uint8_t*>(k.c.codes[feed_values ? 1 : 0]) + feed_at, half, bar);
+      }
+    }
+    feed_slot = feed_slot + 1 == STAGES ? 0 : feed_slot + 1;
+    if (HALVES == 2 || feed_values) {
+      feed_at += half;
+      --feed_left;
+    }
+    feed_values = !feed_values;
+  };
+#pragma unroll 1
+  for (int i = 0; i < STAGES; ++i) feed();
+  int slot = 0;
+  uint32_t parity = 0;
+  const uint32_t ring_at = nb::smem_u32(ring) + lane * 16;
+  // Waits for the copy in `slot`. A copy that never lands ends the warp: the status word is set, whatever is still in
+  // flight gets the same bounded time, and the warp's rows keep what they held.
+  auto landed = [&]() {
+    if (!__all_sync(0xffffffffu, nb::mbar_try_wait(&bars[warp][slot], parity))) {
+      uint32_t i = 0;
+      while (!__all_sync(0xffffffffu, nb::mbar_try_wait(&bars[warp][slot], parity)))
+        if (++i == nb::kSpinLimit) {
+          if (lane == 0) atomicCAS(k.c.status, 0, int(nb::kTimeoutFull));
+          do {
+            for (uint32_t j = 0; j < nb::kSpinLimit; ++j)
+              if (nb::mbar_try_wait(&bars[warp][slot], parity)) break;
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+            if (slot == 0) parity ^= 1;
+          } while (slot != feed_slot);
+          return false;
+        }
+    }
+    return true;
+  };
+  auto release = [&]() {
+    __syncwarp();
+    feed();
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    if (slot == 0) parity ^= 1;
+  };
+
+  long pos = cuts.begin(unit), pos_end = cuts.begin(unit + 1);
+  while (true) {
+    if (pos >= pos_end) {
+      if (unit_next < 0) break;
+      unit = unit_next;
+      unit_next = -1;
+      pos = cuts.begin(unit);
+      pos_end = cuts.begin(unit + 1);
+    }
+    const Run run = run_at(k, cum, lists, pos, pos_end, COLS);
+    const ListWork w = run.w;
+    const int h = run.h, tile = run.tile, b0 = run.b, b1 = run.b + run.blocks;
+    pos += run.blocks;
+    const long lh = long(run.l) * k.c.H + h;
     const float* ksp = k.c.scale[0] + lh * k.c.nb;
     const float* vsp = k.c.scale[1] + lh * k.c.nb;
+    float ks_32 = 0.f, vs_32 = 0.f;            // scales of 32 blocks, one a lane
+    if (b0 + lane < b1) {
+      ks_32 = ksp[b0 + lane];
+      vs_32 = vsp[b0 + lane];
+    }
 
-    uint4 kr[UMAX];
-#pragma unroll
-    for (int u = 0; u < UMAX; ++u) kr[u] = u < U ? ld_stream(kp + (long(b0) * U + u) * 32) : make_uint4(0, 0, 0, 0);
-    float k_scale = ksp[b0], v_scale = vsp[b0];
-
-    // ---- queries: column g of each tile as the B operand, scaled into [1, 2)
-    unsigned qb[NT][PAIRS][2][SP];
-    float qf[NT][2];
+    // ---- queries: column g of each tile as the B operand, scaled by a power of two
+    unsigned qb[NT][PAIRS][2][QS];
+    float qf[NT][2], s_from[NT][2];      // factor on a column's scores; what its sums begin at
     int see[NT][2], seen_least = 0x7fffffff;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -440,28 +606,34 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = 16 * j + (i >> 1) * 8 + 2 * t + (i & 1);
-          x[j][i] = valid && d < D ? load_any(k.a.q, qi + d, k.a.q_type) : 0.f;
+          x[j][i] = valid && d < D ? to_f(reinterpret_cast<const T*>(k.a.q)[qi + d]) : 0.f;
           top = fmaxf(top, fabsf(x[j][i]));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const unsigned ex = min(max(__float_as_uint(top) >> 23, 1u), 253u);       // biased exponent
-      const float down = __uint_as_float((254u - ex) << 23), up = __uint_as_float(ex << 23);
+      constexpr unsigned LIFT = BIASED ? 14 : 0;
+      const unsigned ex = min(max(__float_as_uint(top) >> 23, LIFT + 1u), 253u);       // biased exponent
+      const float down = __uint_as_float((254u + LIFT - ex) << 23), up = __uint_as_float((ex - LIFT) << 23);
+      float q_sum = 0.f;
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float a0 = x[j][2 * i] * down, a1 = x[j][2 * i + 1] * down;
           qb[nt][j][i][0] = pack(a0, a1);
-          if constexpr (SPLIT) {
-            const float2 r = unpack(qb[nt][j][i][0]);
-            qb[nt][j][i][SP - 1] = pack(a0 - r.x, a1 - r.y);
-          }
+          const float2 r = unpack(qb[nt][j][i][0]);
+          if constexpr (QS == 2) qb[nt][j][i][QS - 1] = pack(a0 - r.x, a1 - r.y);
+          if constexpr (BIASED) q_sum += r.x + r.y;
         }
+      if constexpr (BIASED) {
+        q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 1);
+        q_sum += __shfl_xor_sync(0xffffffffu, q_sum, 2);
+      }
       // the score fragment holds columns 2t and 2t + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        qf[nt][i] = __shfl_sync(0xffffffffu, up, (2 * t + i) * 4) * k.a.scale_log2;
+        qf[nt][i] = __shfl_sync(0xffffffffu, up, (2 * t + i) * 4) * k.a.scale_log2 * kUnit;
+        s_from[nt][i] = BIASED ? -128.f / kUnit * __shfl_sync(0xffffffffu, q_sum, (2 * t + i) * 4) : 0.f;
         const int c = tile * COLS + nt * 8 + 2 * t + i, row = c / k.a.group;
         see[nt][i] = row < w.n ? max(0, w.len - (w.n - 1 - row)) : 0;
         if (row < w.n) seen_least = min(seen_least, see[nt][i]);
@@ -469,6 +641,10 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
     }
     seen_least = __reduce_min_sync(0xffffffffu, seen_least);
 
+    // Sums of the weights come from the tensor pipe too: rows of ones, the unused second half of the last pair where
+    // UMAX is odd, a product of their own where it is even.
+    constexpr bool SPARE = UMAX & 1;
+    constexpr unsigned kOnes = 0x3c003c00u;
     float o[PAIRS][NT][4], mx[NT][2], sm[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -481,47 +657,41 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
     }
 
     for (int b = b0; b < b1; ++b) {
-      uint4 vr[UMAX];
-#pragma unroll
-      for (int u = 0; u < UMAX; ++u) vr[u] = u < U ? ld_stream(vp + (long(b) * U + u) * 32) : make_uint4(0, 0, 0, 0);
+      const int in_32 = (b - b0) & 31;
+      if (in_32 == 0 && b != b0 && b + lane < b1) {
+        ks_32 = ksp[b + lane];
+        vs_32 = vsp[b + lane];
+      }
+      const float ks_now = __shfl_sync(0xffffffffu, ks_32, in_32), vs_now = __shfl_sync(0xffffffffu, vs_32, in_32);
       // ---- scores of 64 entries
+      if (!landed()) return;
+      const uint32_t keys_at = ring_at + slot * stage;
       float s[NT][4][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][m][i] = 0.f;
-#pragma unroll
       for (int j = 0; j < PAIRS; ++j) {
-        const unsigned x[4] = {kr[2 * j].x, kr[2 * j].y, kr[2 * j].z, kr[2 * j].w};
-        unsigned y[4] = {0, 0, 0, 0};
-        if (2 * j + 1 < UMAX) {
-          const uint4 z = kr[2 * j + 1 < UMAX ? 2 * j + 1 : 0];
-          y[0] = z.x; y[1] = z.y; y[2] = z.z; y[3] = z.w;
-        }
+        const uint4 z0 = 2 * j < U ? lds(keys_at + 2 * j * 512) : make_uint4(0, 0, 0, 0);
+        uint4 z1 = make_uint4(0, 0, 0, 0);
+        if (2 * j + 1 < UMAX && 2 * j + 1 < U) z1 = lds(keys_at + (2 * j + 1) * 512);
+        const unsigned x[4] = {z0.x, z0.y, z0.z, z0.w}, y[4] = {z1.x, z1.y, z1.z, z1.w};
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           unsigned a0, a1, a2 = 0, a3 = 0;
-          widen<CODE>(x[m], a0, a1);
-          if (2 * j + 1 < UMAX) widen<CODE>(y[m], a2, a3);
+          widen<CODE, RAW>(x[m], a0, a1);
+          if (2 * j + 1 < UMAX) widen<CODE, RAW>(y[m], a2, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = 0; q < SP; ++q) mma(s[nt][m], a0, a1, a2, a3, qb[nt][j][0][q], qb[nt][j][1][q]);
+            for (int q = 0; q < QS; ++q) {
+              if (j == 0 && q == 0) mma_from(s[nt][m], a0, a1, a2, a3, qb[nt][j][0][q], qb[nt][j][1][q], s_from[nt][0], s_from[nt][1]);
+              else mma(s[nt][m], a0, a1, a2, a3, qb[nt][j][0][q], qb[nt][j][1][q]);
+            }
         }
       }
-      const float ks_now = k_scale, vs_now = v_scale;
-      if (b + 1 < b1) {
-#pragma unroll
-        for (int u = 0; u < UMAX; ++u) kr[u] = u < U ? ld_stream(kp + (long(b + 1) * U + u) * 32) : make_uint4(0, 0, 0, 0);
-        k_scale = ksp[b + 1];
-        v_scale = vsp[b + 1];
-      }
-      // ---- softmax; columns whose view ends inside (or before) this block take the masked form
+      if (HALVES == 1) release();
+      // ---- softmax; a block in which some column's view ends takes the masked form
       const bool masked = (b + 1) * kBlock > seen_least;
-      unsigned pb[NT][4][2][SP];
-      float keep[NT][2], vs_col[NT][2];
+      float f[NT][2], vs_col[NT][2];
+      bool grows = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (masked) {
@@ -531,123 +701,181 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
             for (int i = 0; i < 4; ++i)
               if (b * kBlock + 16 * m + (i >> 1) * 8 + g >= see[nt][i & 1]) s[nt][m][i] = -INFINITY;
         }
-        float off[2], f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          f[i] = qf[nt][i] * ks_now;
-          float top = fmaxf(fmaxf(fmaxf(s[nt][0][i], s[nt][0][2 + i]), fmaxf(s[nt][1][i], s[nt][1][2 + i])),
-                            fmaxf(fmaxf(s[nt][2][i], s[nt][2][2 + i]), fmaxf(s[nt][3][i], s[nt][3][2 + i])));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-          const float now = fmaxf(mx[nt][i], top * f[i]);
-          keep[nt][i] = now == mx[nt][i] ? 1.f : ex2(mx[nt][i] - now);
-          off[i] = kShift - now;
-          mx[nt][i] = now;
-          vs_col[nt][i] = !masked || b * kBlock < see[nt][i] ? vs_now : 0.f;
+          f[nt][i] = qf[nt][i] * ks_now;
+          vs_col[nt][i] = vs_now;
+          if (masked && b * kBlock >= see[nt][i]) vs_col[nt][i] = 0.f;
+          grows |= tile_max(s[nt], i) * f[nt][i] > mx[nt][i] + kSlack;
         }
-        float add[2] = {0.f, 0.f};
+      }
+      // The running maximum follows a column's true one with a lag of at most kSlack, so most blocks leave it (and the
+      // accumulators) alone: one vote instead of six shuffles and a rescaling.
+      if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          float p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = ex2(fmaf(s[nt][m][i], f[i & 1], off[i & 1]));
-            if (masked && s[nt][m][i] == -INFINITY && b * kBlock + 16 * m + (i >> 1) * 8 + g >= see[nt][i & 1]) p[i] = 0.f;
-          }
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const unsigned hi = pack(p[2 * i], p[2 * i + 1]);
-            const float2 r = unpack(hi);
-            pb[nt][m][i][0] = transpose8x8(hi);
-            if constexpr (SPLIT) {
-              pb[nt][m][i][SP - 1] = transpose8x8(pack(p[2 * i] - r.x, p[2 * i + 1] - r.y));
-              add[0] += p[2 * i];
-              add[1] += p[2 * i + 1];
-            } else {
-              add[0] += r.x;
-              add[1] += r.y;
+            float top = tile_max(s[nt], i);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float now = fmaxf(mx[nt][i], top * f[nt][i]), keep = now == mx[nt][i] ? 1.f : ex2(mx[nt][i] - now);
+            mx[nt][i] = now;
+            sm[nt][i] *= keep;
+#pragma unroll
+            for (int j = 0; j < PAIRS; ++j) {
+              o[j][nt][i] *= keep;
+              o[j][nt][2 + i] *= keep;
             }
           }
+      }
+      unsigned pb[NT][4][2][PS];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 off = make_float2(kShift - mx[nt][0], kShift - mx[nt][1]);
+        const float2 by = make_float2(f[nt][0], f[nt][1]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float2 e = fma2(make_float2(s[nt][m][2 * i], s[nt][m][2 * i + 1]), by, off);
+            s[nt][m][2 * i] = ex2(e.x);
+            s[nt][m][2 * i + 1] = ex2(e.y);
+          }
+        if (masked) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (b * kBlock + 16 * m + (i >> 1) * 8 + g >= see[nt][i & 1]) s[nt][m][i] = 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) sm[nt][i] = sm[nt][i] * keep[nt][i] + add[i];
-      }
-      if (CODE != 0 && (b + 1) * kBlock > w.len) {      // entries that the list does not hold may be any bytes, NaN codes too
+        for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int u = 0; u < UMAX; ++u) {
-          unsigned* words = reinterpret_cast<unsigned*>(&vr[u]);
+          for (int i = 0; i < 2; ++i) {
+            const unsigned hi = pack(s[nt][m][2 * i], s[nt][m][2 * i + 1]);
+            pb[nt][m][i][0] = transpose8x8(hi);
+            if constexpr (PS == 2) {
+              const float2 r = unpack(hi);
+              pb[nt][m][i][PS - 1] = transpose8x8(pack(s[nt][m][2 * i] - r.x, s[nt][m][2 * i + 1] - r.y));
+            }
+          }
+      }
+      // ---- output of these entries
+      if (HALVES == 1 && !landed()) return;
+      const uint32_t values_at = ring_at + slot * stage + (HALVES - 1) * half;
+      const bool past_end = CODE != 0 && (b + 1) * kBlock > w.len;
+      // (the last pair first: its spare rows bring the sums of the weights, from which the others' bias follows)
+      float ones[NT][2];
+      if constexpr (!SPARE) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float acc[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int q = 0; q < PS; ++q) {
+              if (m == 0 && q == 0) mma_from(acc, kOnes, kOnes, kOnes, kOnes, pb[nt][m][0][q], pb[nt][m][1][q], 0.f, 0.f);
+              else mma(acc, kOnes, kOnes, kOnes, kOnes, pb[nt][m][0][q], pb[nt][m][1][q]);
+            }
+          ones[nt][0] = acc[0];
+          ones[nt][1] = acc[1];
+        }
+      }
+      float v_from[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v_from[nt][i] = BIASED && !SPARE ? -128.f / kUnit * ones[nt][i] : 0.f;
+#pragma unroll
+      for (int j = PAIRS - 1; j >= 0; --j) {
+        float acc[NT][4];
+        const uint4 z0 = 2 * j < U ? lds(values_at + 2 * j * 512) : make_uint4(0, 0, 0, 0);
+        uint4 z1 = make_uint4(0, 0, 0, 0);
+        if (2 * j + 1 < UMAX && 2 * j + 1 < U) z1 = lds(values_at + (2 * j + 1) * 512);
+        unsigned x[4] = {z0.x, z0.y, z0.z, z0.w}, y[4] = {z1.x, z1.y, z1.z, z1.w};
+        if (past_end) {      // entries that the list does not hold may be any bytes, NaN codes too
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             unsigned keep_bytes = 0;
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               if (b * kBlock + 16 * m + (q >> 1) * 8 + 2 * t + (q & 1) < w.len) keep_bytes |= 0xffu << (8 * q);
-            words[m] &= keep_bytes;
+            x[m] &= keep_bytes;
+            y[m] &= keep_bytes;
           }
-        }
-      }
-      // ---- output of these entries
-#pragma unroll
-      for (int j = 0; j < PAIRS; ++j) {
-        float acc[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-        const unsigned x[4] = {vr[2 * j].x, vr[2 * j].y, vr[2 * j].z, vr[2 * j].w};
-        unsigned y[4] = {0, 0, 0, 0};
-        if (2 * j + 1 < UMAX) {
-          const uint4 z = vr[2 * j + 1 < UMAX ? 2 * j + 1 : 0];
-          y[0] = z.x; y[1] = z.y; y[2] = z.z; y[3] = z.w;
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          unsigned a0, a1 = 0, a2, a3 = 0;
-          widen<CODE>(x[m], a0, a2);
-          if (2 * j + 1 < UMAX) widen<CODE>(y[m], a1, a3);
+          unsigned a0, a1 = kOnes, a2, a3 = kOnes;
+          widen<CODE, RAW>(x[m], a0, a2);
+          if (2 * j + 1 < UMAX) widen<CODE, RAW>(y[m], a1, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int q = 0; q < SP; ++q) mma(acc[nt], a0, a1, a2, a3, pb[nt][m][0][q], pb[nt][m][1][q]);
+            for (int q = 0; q < PS; ++q) {
+              if (m == 0 && q == 0) mma_from(acc[nt], a0, a1, a2, a3, pb[nt][m][0][q], pb[nt][m][1][q], v_from[nt][0], v_from[nt][1]);
+              else mma(acc[nt], a0, a1, a2, a3, pb[nt][m][0][q], pb[nt][m][1][q]);
+            }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          if (SPARE && j == PAIRS - 1) {
+            ones[nt][0] = acc[nt][2];
+            ones[nt][1] = acc[nt][3];
+            if constexpr (BIASED) {
+              v_from[nt][0] = -128.f / kUnit * ones[nt][0];
+              v_from[nt][1] = -128.f / kUnit * ones[nt][1];
+              acc[nt][0] += v_from[nt][0];
+              acc[nt][1] += v_from[nt][1];
+            }
+          }
+          const float2 vs = make_float2(vs_col[nt][0], vs_col[nt][1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) o[j][nt][i] = fmaf(o[j][nt][i], keep[nt][i & 1], acc[nt][i] * vs_col[nt][i & 1]);
+          for (int q = 0; q < 2; ++q) {
+            if (q == 1 && SPARE && j == PAIRS - 1) continue;
+            const float2 into = fma2(make_float2(acc[nt][2 * q], acc[nt][2 * q + 1]), vs, make_float2(o[j][nt][2 * q], o[j][nt][2 * q + 1]));
+            o[j][nt][2 * q] = into.x;
+            o[j][nt][2 * q + 1] = into.y;
+          }
+        }
       }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        sm[nt][0] += ones[nt][0];
+        sm[nt][1] += ones[nt][1];
+      }
+      release();
     }
 
     // ---- the piece's result
     const bool whole = b0 == 0 && b1 == w.nb;
-    float* slot = k.ws + long(2 * worker + (b0 == 0 ? 1 : 0)) * COLS * (8 * U + 2);
+    float* to_piece = k.ws + long(2 * unit + (b0 == 0 ? 1 : 0)) * COLS * (8 * U + 2);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float z = sm[nt][i];
-        z += __shfl_xor_sync(0xffffffffu, z, 4);
-        z += __shfl_xor_sync(0xffffffffu, z, 8);
-        z += __shfl_xor_sync(0xffffffffu, z, 16);
+        const float z = sm[nt][i];
         const int in_tile = nt * 8 + 2 * t + i, c = tile * COLS + in_tile, row = c / k.a.group;
         if (row >= w.n) continue;
         if (whole) {
-          const float inv = z == 0.f ? 0.f : 1.f / z;
+          const float inv = z == 0.f ? 0.f : kUnit / z;
           const long at = long(w.s0 + row) * k.a.o_row + long(h * k.a.group + c - row * k.a.group) * k.a.o_head;
 #pragma unroll
           for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
               const int d = 16 * j + 8 * q + g;
-              if (d < D) store_any(k.a.out, at + d, k.a.q_type, o[j][nt][2 * q + i] * inv);
+              if (d < D) reinterpret_cast<T*>(k.a.out)[at + d] = from_f<T>(o[j][nt][2 * q + i] * inv);
             }
         } else {
-          float* to = slot + in_tile * (8 * U + 2);
+          float* to = to_piece + in_tile * (8 * U + 2);
 #pragma unroll
           for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
-              if (16 * j + 8 * q + g < 8 * U) to[16 * j + 8 * q + g] = o[j][nt][2 * q + i];
+              if (16 * j + 8 * q + g < 8 * U) to[16 * j + 8 * q + g] = o[j][nt][2 * q + i] * kUnit;
           if (g == 0) {
             to[8 * U] = mx[nt][i];
             to[8 * U + 1] = z;
@@ -657,44 +885,51 @@ __global__ void __launch_bounds__(kWarps * 32) attn_kernel(const Attn k) {
   }
 }
 
-// One CTA for each (row, query head): adds the pieces of its task in their order. Rows whose task was one piece are
-// done already. Rows behind the last list become zeros when `zero_tail` is set.
-__global__ void __launch_bounds__(kWarps * 32) attn_join(const Attn k, int cols) {
-  const int row = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Adds the pieces of each (row, query head) whose task was cut, in their order. TEAM warps share an item: 4 where there
+// are few items (their tasks are cut into many pieces then), else 1. Rows behind the last list become zeros when
+// `zero_tail` is set. Launched so that it starts under the main kernel's end: up to the wait it reads the caller's
+// tensors only.
+template <int TEAM>
+__global__ void __launch_bounds__(kJoin * 32) attn_join(const Attn k, int cols) {
+  __shared__ float red[kJoin], sums[kJoin], acc_s[kJoin][128];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM, heads = k.c.H * k.a.group;
+  const long item = blockIdx.x * long(kJoin / TEAM) + warp / TEAM;
+  const int row = int(item / heads), head = int(item - long(row) * heads);
   const int L = k.c.L, D = k.c.D, width = 8 * k.c.U + 2;
-  if (row < k.a.seg[0]) return;
+  const int seg_begin = k.a.seg[0], seg_end = k.a.seg[L];
+  bool live = item < long(k.a.rows) * heads && row >= seg_begin && row < seg_end;
+  const bool tail = k.a.zero_tail && item < long(k.a.rows) * heads && row >= seg_end;
   const long at = long(row) * k.a.o_row + long(head) * k.a.o_head;
-  if (row >= k.a.seg[L]) {
-    if (k.a.zero_tail)
-      for (int d = threadIdx.x; d < D; d += blockDim.x) store_any(k.a.out, at + d, k.a.q_type, 0.f);
-    return;
-  }
-  const int l = find_list(k.a.seg, L, row);
-  const ListWork w = list_work(k, l, cols);
-  if (row < w.s0 || row >= w.s0 + w.n) {      // bounds that the main kernel refused
-    for (int d = threadIdx.x; d < D; d += blockDim.x) store_any(k.a.out, at + d, k.a.q_type, 0.f);
-    return;
-  }
-  const long total = k.cum[L];
-  const int P = pieces(total, k.workers, k.min_blocks);
+  const int l = find_list(k.a.seg, L, live ? row : seg_begin);
+  const ListWork w = list_work(k, l, seg_end, cols);
+  const bool refused = live && (row < w.s0 || row >= w.s0 + w.n);      // bounds that the main kernel refused
+  if (tail || refused)
+    for (int d = lane + 32 * member; d < D; d += 32 * TEAM) store_any(k.a.out, at + d, k.a.q_type, 0.f);
+  live = live && !refused;
   const int h = head / k.a.group, col = (row - w.s0) * k.a.group + head - h * k.a.group;
-  const long begin = k.cum[l] + (h * w.tiles + col / cols) * w.nb;
-  const int w0 = int(((begin + 1) * P - 1) / total), w1 = int(((begin + w.nb) * P - 1) / total);
-  if (w0 == w1) return;
-  auto piece = [&](int i) { return k.ws + (long(2 * (w0 + i) + (i == 0 ? 1 : 0)) * cols + col % cols) * width; };
-  const int n = w1 - w0 + 1;
-  __shared__ float red[kWarps], sums[kWarps], acc_s[kWarps][128];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int u0 = 0, n = 0;
+  if (live) {
+    const Cuts cuts(k, k.cum[L]);
+    const long begin = k.cum[l] + (long(h) * w.tiles + col / cols) * w.nb;
+    u0 = cuts.of(begin);
+    n = cuts.of(begin + w.nb - 1) - u0 + 1;
+  }
+  if (TEAM == 1 ? n <= 1 : __syncthreads_and(n <= 1)) return;
+  auto piece = [&](int i) { return k.ws + (long(2 * (u0 + i) + (i == 0 ? 1 : 0)) * cols + col % cols) * width; };
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) top = fmaxf(top, piece(i)[8 * k.c.U]);
+  for (int i = lane + 32 * member; i < n; i += 32 * TEAM) top = fmaxf(top, piece(i)[8 * k.c.U]);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-  if (lane == 0) red[warp] = top;
-  __syncthreads();
+  if constexpr (TEAM > 1) {
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) top = fmaxf(top, red[i]);
+    for (int i = 0; i < TEAM; ++i) top = fmaxf(top, red[i]);
+  }
   float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll 4
-  for (int i = warp; i < n; i += kWarps) {
+  for (int i = member; i < n; i += TEAM) {
     const float* from = piece(i);
     const float m = from[8 * k.c.U], f = m == top ? 1.f : ex2(m - top);
     sum += f * from[8 * k.c.U + 1];
@@ -702,40 +937,51 @@ __global__ void __launch_bounds__(kWarps * 32) attn_join(const Attn k, int cols)
     for (int q = 0; q < 4; ++q)
       if (lane + 32 * q < D) acc[q] += f * from[lane + 32 * q];
   }
+  if constexpr (TEAM > 1) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) acc_s[warp][lane + 32 * q] = acc[q];
-  if (lane == 0) sums[warp] = sum;
-  __syncthreads();
-  float z = 0.f;
+    for (int q = 0; q < 4; ++q) acc_s[warp][lane + 32 * q] = acc[q];
+    if (lane == 0) sums[warp] = sum;
+    __syncthreads();
+    sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) z += sums[i];
-  const float inv = z == 0.f ? 0.f : 1.f / z;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float x = 0.f;
+    for (int i = 0; i < TEAM; ++i) sum += sums[i];
+    const int d = threadIdx.x;       // (128 threads, at most 128 dims)
+    if (d < D) {
+      float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) x += acc_s[i][d];
-    store_any(k.a.out, at + d, k.a.q_type, x * inv);
+      for (int i = 0; i < TEAM; ++i) x += acc_s[i][d];
+      store_any(k.a.out, at + d, k.a.q_type, sum == 0.f ? 0.f : x / sum);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (lane + 32 * q < D) store_any(k.a.out, at + lane + 32 * q, k.a.q_type, sum == 0.f ? 0.f : acc[q] / sum);
   }
 }
 
 // ------------------------------------------------------------------------------------------------------ launches
 using AttnFn = void (*)(const Attn);
 
+template <int UMAX, int NT, int CODE>
+AttnFn pick_type(int type) {
+  return type == 0 ? attn_kernel<UMAX, NT, CODE, __nv_bfloat16> : type == 1 ? attn_kernel<UMAX, NT, CODE, __half> : attn_kernel<UMAX, NT, CODE, float>;
+}
 template <int UMAX, int NT>
-AttnFn pick_code(int code, bool split) {
-  if (code == 0) return split ? attn_kernel<UMAX, NT, 0, true> : attn_kernel<UMAX, NT, 0, false>;
-  return split ? attn_kernel<UMAX, NT, 1, true> : attn_kernel<UMAX, NT, 1, false>;
+AttnFn pick_code(int code, int type) {
+  return code == 0 ? pick_type<UMAX, NT, 0>(type) : pick_type<UMAX, NT, 1>(type);
 }
 
-// Column tiles of 8: one for single tokens, more when several rows or shared heads bring more columns (a converted
-// block then serves them all); wide heads take at most two because their accumulators fill the registers.
-int tiles_for(int U, int columns) { return columns <= 8 ? 1 : (U <= 8 && columns > 16 ? 4 : 2); }
+// Column tiles of 8: one for single tokens, two when several rows or shared heads bring more columns (a converted
+// block then serves both); four would not fit the registers of the wider heads.
+int tiles_for(int columns) { return columns <= 8 ? 1 : 2; }
 
-AttnFn pick(int U, int nt, int code, bool split) {
-  if (U <= 5) return nt == 1 ? pick_code<5, 1>(code, split) : nt == 2 ? pick_code<5, 2>(code, split) : pick_code<5, 4>(code, split);
-  if (U <= 8) return nt == 1 ? pick_code<8, 1>(code, split) : nt == 2 ? pick_code<8, 2>(code, split) : pick_code<8, 4>(code, split);
-  if (U <= 10) return nt == 1 ? pick_code<10, 1>(code, split) : pick_code<10, 2>(code, split);
-  return nt == 1 ? pick_code<16, 1>(code, split) : pick_code<16, 2>(code, split);
+int width_of(int U) { return U <= 5 ? 5 : U <= 8 ? 8 : U <= 10 ? 10 : 16; }
+
+AttnFn pick(int U, int nt, int code, int type) {
+  if (U <= 5) return nt == 1 ? pick_code<5, 1>(code, type) : pick_code<5, 2>(code, type);
+  if (U <= 8) return nt == 1 ? pick_code<8, 1>(code, type) : pick_code<8, 2>(code, type);
+  if (U <= 10) return nt == 1 ? pick_code<10, 1>(code, type) : pick_code<10, 2>(code, type);
+  return nt == 1 ? pick_code<16, 1>(code, type) : pick_code<16, 2>(code, type);
 }
 
 int multiprocessors() {
@@ -744,9 +990,27 @@ int multiprocessors() {
   return sms;
 }
 
-constexpr int kMaxCtas = 12;      // CTAs of attn_kernel on one SM that the workspace is sized for
+int variant(int U, int nt, int code, int type) {
+  const int w = U <= 5 ? 0 : U <= 8 ? 1 : U <= 10 ? 2 : 3;
+  return ((w * 2 + (nt - 1)) * 2 + code) * 3 + type;
+}
+
+// Lets `fn` use up to `kSmem` bytes of dynamic shared memory (once for each device and variant: the call takes a
+// microsecond and the answer does not change).
+constexpr int kSmem = 226 * 1024;
+cudaError_t allow_smem(AttnFn fn, int which) {
+  constexpr int kDevices = 16;
+  static std::atomic<bool> done[kDevices][48];
+  int dev = 0;
+  cudaError_t rc = cudaGetDevice(&dev);
+  if (rc != cudaSuccess || (dev < kDevices && done[dev][which].load(std::memory_order_relaxed))) return rc;
+  rc = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (rc == cudaSuccess && dev < kDevices) done[dev][which].store(true, std::memory_order_relaxed);
+  return rc;
+}
 
 long slot_floats(int U, int cols) { return long(cols) * (8 * U + 2); }
+long workers_of(int U, int nt) { return long(multiprocessors()) * warps_of(width_of(U), nt); }
 
 
 // The widest vector (at most 16 bytes) that divides the head and that every row start is aligned to.
@@ -835,31 +1099,29 @@ int nb_kv8_read(const nb_kv8_cache* c, const nb_kv8_rows* p, int type, cudaStrea
 // Bytes of workspace that an attention call over heads of D dims takes for `columns` query columns a list and head.
 long nb_kv8_attention_workspace(int D, int columns) {
   using namespace nbk;
-  const int U = (D + 7) / 8, nt = tiles_for(U, columns);
-  return long(multiprocessors()) * kMaxCtas * kWarps * 2 * slot_floats(U, 8 * nt) * 4 + (kMaxLists + 2) * 8;
+  const int U = (D + 7) / 8, nt = tiles_for(columns);
+  return 16 + (kMaxLists + 2) * 8 + workers_of(U, nt) * (1 + kShares) * 2 * slot_floats(U, 8 * nt) * 4;
 }
 
 int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long ws_bytes, cudaStream_t st) {
   using namespace nbk;
-  if (bad_cache(c) || a->rows < 0 || a->group < 1 || long(c->H) * a->group > 65535) return -1;
+  if (bad_cache(c) || a->rows < 0 || a->group < 1) return -1;
   // (a list's tasks are counted in 32 bits)
   if (long(c->H) * ((long(a->rows) * a->group + 7) / 8) * c->nb > 0x7fffffffl) return -3;
   if (a->rows == 0) return 0;
-  const int sms = multiprocessors();
   const long columns = long(a->max_rows) * a->group;
-  const int nt = tiles_for(c->U, columns > 1024 ? 1024 : int(columns)), cols = 8 * nt;
-  AttnFn fn = pick(c->U, nt, c->code, a->q_type == 2);
-  const int L_smem = c->L < kMaxLists ? c->L : kMaxLists;
-  int occ = 1;
-  cudaError_t rc = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, fn, kWarps * 32, (L_smem + 1) * sizeof(long));
+  const int nt = tiles_for(columns > 1024 ? 1024 : int(columns)), cols = 8 * nt, width = width_of(c->U);
+  AttnFn fn = pick(c->U, nt, c->code, a->q_type);
+  const int warps = warps_of(width, nt), L_smem = c->L < kMaxLists ? c->L : kMaxLists;
+  const size_t smem = size_t(warps) * stages_of(width) * halves_of(width) * c->U * 512 + 8 + L_smem * 20;
+  cudaError_t rc = allow_smem(fn, variant(c->U, nt, c->code, a->q_type));
   if (rc != cudaSuccess) return int(rc);
-  occ = occ < 1 ? 1 : (occ > kMaxCtas ? kMaxCtas : occ);
+  const int sms = multiprocessors(), all = sms * warps;
   Attn k;
-  k.cum = reinterpret_cast<long*>(ws);
+  k.next = reinterpret_cast<int*>(ws);
+  k.cum = reinterpret_cast<long*>(reinterpret_cast<char*>(ws) + 16);
   k.ws = reinterpret_cast<float*>(k.cum + kMaxLists + 2);
-  k.min_blocks = 1;
-  k.workers = sms * occ * kWarps;
-  if (long(k.workers) * 2 * slot_floats(c->U, cols) * 4 + (kMaxLists + 2) * 8 > ws_bytes) return -2;
+  if (nb_kv8_attention_workspace(c->D, nt * 8) > ws_bytes) return -2;
   for (int l0 = 0; l0 < c->L; l0 += kMaxLists) {      // (more lists than one launch holds: slices, in stream order)
     k.c = *c;
     k.a = *a;
@@ -871,11 +1133,27 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
     }
     k.a.seg += l0;
     k.a.len += l0;
-    const bool last = l0 + k.c.L >= c->L;
-    k.a.zero_tail = a->zero_tail && last;
-    fn<<<sms * occ, kWarps * 32, (k.c.L + 1) * sizeof(long), st>>>(k);
-    attn_join<<<dim3(a->rows, c->H * a->group), kWarps * 32, 0, st>>>(k, cols);
-    rc = cudaGetLastError();
+    k.a.zero_tail = a->zero_tail && l0 + k.c.L >= c->L;
+    // the most blocks that this slice can have, as far as the host knows
+    const long most_tasks = std::min(long(a->rows) * a->group, std::min(long(a->rows), long(k.c.L)) * ((columns + cols - 1) / cols)) * c->H;
+    k.dynamic = most_tasks * c->nb >= long(kLong) * all;
+    if (k.dynamic && (rc = cudaMemsetAsync(k.next, 0, sizeof(int), st)) != cudaSuccess) return int(rc);
+    const int grid = k.dynamic ? sms : int(std::min(long(sms), std::max(most_tasks * c->nb, 1l)));
+    k.workers = grid * warps;
+    fn<<<grid, warps * 32, smem, st>>>(k);
+    if ((rc = cudaGetLastError()) != cudaSuccess) return int(rc);
+    const long items = long(a->rows) * c->H * a->group;
+    const bool teams = items <= 16l * sms;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(teams ? items : (items + kJoin - 1) / kJoin));
+    cfg.blockDim = dim3(kJoin * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    rc = teams ? cudaLaunchKernelEx(&cfg, attn_join<kJoin>, (const Attn)k, cols) : cudaLaunchKernelEx(&cfg, attn_join<1>, (const Attn)k, cols);
     if (rc != cudaSuccess) return int(rc);
   }
   return 0;

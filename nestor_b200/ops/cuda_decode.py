@@ -14,13 +14,14 @@ from nestor_b200.ops.decode import BLOCK, FLOATS, KV8Cache
 
 
 class CacheArgs(C.Structure):
-    _fields_ = [("codes", C.c_void_p * 2), ("scale", C.c_void_p * 2), ("open", C.c_void_p * 2), ("status", C.c_void_p),
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("k_open", C.c_void_p), ("v_open", C.c_void_p), ("status", C.c_void_p),
                 ("L", C.c_int), ("H", C.c_int), ("nb", C.c_int), ("D", C.c_int), ("U", C.c_int), ("code", C.c_int), ("type", C.c_int)]
 
 
-class RowArgs(C.Structure):
-    _fields_ = [("src", C.c_void_p * 2), ("row_stride", C.c_long * 2), ("head_stride", C.c_long * 2), ("dst", C.c_void_p * 2),
-                ("seg", C.c_void_p), ("start", C.c_void_p), ("rows", C.c_int), ("max_rows", C.c_int)]
+class RowArgs(C.Structure):      # (pairs of the C structure, keys then values, are two fields here: cheaper to fill)
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_row", C.c_long), ("v_row", C.c_long), ("k_head", C.c_long),
+                ("v_head", C.c_long), ("k_out", C.c_void_p), ("v_out", C.c_void_p), ("seg", C.c_void_p), ("start", C.c_void_p), ("rows", C.c_int), ("max_rows", C.c_int)]
 
 
 class AttentionArgs(C.Structure):
@@ -35,6 +36,7 @@ class VerifyArgs(C.Structure):
                 ("q_row", C.c_long), ("B", C.c_int), ("n", C.c_int), ("V", C.c_int), ("type", C.c_int), ("tokens_64", C.c_int)]
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _ready = None
 
 
@@ -59,11 +61,13 @@ def _L():
 def _launch(fn, device: torch.device, *args, launches: int = 1) -> None:
     """Call an entry point with the current stream of ``device`` (which need not be the current device)."""
 
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+    # (the raw-stream query costs a tenth of torch.cuda.current_stream(), which builds a Stream object)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"{fn.__name__} failed with code {rc}")
     _lib.count_launch(launches)
@@ -72,10 +76,9 @@ def _launch(fn, device: torch.device, *args, launches: int = 1) -> None:
 def _cache_args(c: KV8Cache) -> CacheArgs:
     a = c.__dict__.get("_args")          # (the fields are frozen: one argument block serves every call)
     if a is None:
-        L, H, nb, U, _ = c.k_codes.shape
-        a = CacheArgs((c.k_codes.data_ptr(), c.v_codes.data_ptr()), (c.k_scale.data_ptr(), c.v_scale.data_ptr()),
-                      (c.k_open.data_ptr(), c.v_open.data_ptr()), _lib.status_word(c.device).data_ptr(), L, H, nb, c.head_dim, U,
-                      0 if c.dtype == torch.int8 else 1, FLOATS[c.k_open.dtype])
+        a = CacheArgs(c.k_codes.data_ptr(), c.v_codes.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.k_open.data_ptr(),
+                      c.v_open.data_ptr(), _lib.status_word(c.device).data_ptr(), c.lists, c.heads, c.blocks, c.head_dim, c.units,
+                      0 if c.dtype == torch.int8 else 1, FLOATS[c.open_dtype])
         c.__dict__["_args"] = a
     return a
 
@@ -89,8 +92,9 @@ def kv8_append(cache: KV8Cache, k: Tensor, v: Tensor, seg_start: Tensor, start: 
     if k.shape[0] == 0:
         return
     k, v = _rows(k), _rows(v)
-    a = RowArgs((k.data_ptr(), v.data_ptr()), (k.stride(0), v.stride(0)), (k.stride(1), v.stride(1)), (None, None),
-                seg_start.data_ptr(), start.data_ptr(), k.shape[0], max_rows)
+    (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
+    a = RowArgs(k.data_ptr(), v.data_ptr(), k_row, v_row, k_head, v_head, None, None, seg_start.data_ptr(), start.data_ptr(),
+                k.shape[0], max_rows)
     _launch(_L().nb_kv8_append, cache.device, _cache_args(cache), a)
 
 
@@ -105,11 +109,12 @@ def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype
     k = torch.empty(rows, cache.heads, cache.head_dim, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
     if rows:
-        a = RowArgs((None, None), (0, 0), (0, 0), (k.data_ptr(), v.data_ptr()), seg_start.data_ptr(), start.data_ptr(), rows, max_rows)
+        a = RowArgs(None, None, 0, 0, 0, 0, k.data_ptr(), v.data_ptr(), seg_start.data_ptr(), start.data_ptr(), rows, max_rows)
         _launch(_L().nb_kv8_read, cache.device, _cache_args(cache), a, FLOATS[dtype])
     return k, v
 
 
+LOG2E = math.log2(math.e)
 _workspace: dict[tuple[int, int, int], int] = {}
 
 
@@ -122,6 +127,8 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     if q.shape[0] == 0:
         return out
     q = _rows(q)
+    q_row, q_head, _ = q.stride()
+    o_row, o_head, _ = out.stride()
     L = _L()
     group = q.shape[1] // cache.heads
     key = (cache.head_dim, min(max_rows * group, 32), cache.device.index)
@@ -131,8 +138,8 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
             size = _workspace[key] = L.nb_kv8_attention_workspace(key[0], key[1])
     # (allocated for this call on this stream: two streams, or two captured graphs, never share it)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device)
-    a = AttentionArgs(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1), seg_start.data_ptr(),
-                      lengths.data_ptr(), q.shape[0], max_rows, group, FLOATS[q.dtype], int(not given), scale * math.log2(math.e))
+    a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(),
+                      lengths.data_ptr(), q.shape[0], max_rows, group, FLOATS[q.dtype], int(not given), scale * LOG2E)
     _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, ws.data_ptr(), size, launches=2)
     return out
 

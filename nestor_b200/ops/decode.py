@@ -38,6 +38,7 @@ class KV8Cache:
         k_scale, v_scale: ``[L, H, blocks]`` fp32.
         k_open, v_open: ``[L, H, 2, 64, head_dim]`` originals of the youngest two blocks (block ``b`` in slot ``b % 2``),
             in the dtype of the rows that are appended (bf16, fp16 or fp32).
+        lists, heads, blocks, units, capacity, head_dim, device, dtype, open_dtype: what the tensors' shapes say.
 
     How many entries each list holds is not part of the cache: the caller keeps ``lengths [L]`` (int32, on the device)
     and passes it, so stepping back is a smaller number plus :func:`kv8_truncate`.
@@ -51,32 +52,29 @@ class KV8Cache:
     v_open: Tensor
 
     def __post_init__(self) -> None:
-        kc, ks, ko = self.k_codes, self.k_scale, self.k_open
-        if kc.dtype not in CODE_MAX or self.v_codes.dtype != kc.dtype:
-            raise ValueError(f"cache codes are int8 or float8_e4m3fn (keys and values alike), got {kc.dtype} and {self.v_codes.dtype}")
-        if ko.dtype not in FLOATS or self.v_open.dtype != ko.dtype:
-            raise ValueError(f"the kept originals are bfloat16, float16 or float32 (keys and values alike), got {ko.dtype} and {self.v_open.dtype}")
-        if kc.dim() != 5 or ko.dim() != 5:
+        kc, vc, ks, vs, ko, vo = self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_open, self.v_open
+        code, kind = kc.dtype, ko.dtype
+        if code not in CODE_MAX or vc.dtype != code:
+            raise ValueError(f"cache codes are int8 or float8_e4m3fn (keys and values alike), got {code} and {vc.dtype}")
+        if kind not in FLOATS or vo.dtype != kind:
+            raise ValueError(f"the kept originals are bfloat16, float16 or float32 (keys and values alike), got {kind} and {vo.dtype}")
+        if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+            raise ValueError("cache scales are float32")
+        shape, held = kc.shape, ko.shape
+        if len(shape) != 5 or len(held) != 5:
             raise ValueError("cache codes are [L, H, blocks, units, 512], originals [L, H, 2, 64, head_dim]")
-        L, H, nb, U, _ = kc.shape
-        D = ko.shape[-1]
+        L, H, nb, U, _ = shape
+        D = held[4]
         if min(L, H, nb) < 1 or not 1 <= D <= MAX_HEAD_DIM or U != -(-D // 8):
             raise ValueError(f"cache of {L} lists x {H} heads x {nb} blocks x {U} units for head_dim {D}: needs at least one of "
                              f"each, head_dim in 1..{MAX_HEAD_DIM} and ceil(head_dim / 8) units")
-        for t, shape in ((kc, (L, H, nb, U, 512)), (self.v_codes, (L, H, nb, U, 512)), (ks, (L, H, nb)), (self.v_scale, (L, H, nb)),
-                         (ko, (L, H, 2, BLOCK, D)), (self.v_open, (L, H, 2, BLOCK, D))):
-            if t.shape != shape or not t.is_contiguous() or t.device != kc.device:
+        device = kc.device
+        for t, want in ((kc, (L, H, nb, U, 512)), (vc, shape), (ks, (L, H, nb)), (vs, (L, H, nb)), (ko, (L, H, 2, BLOCK, D)), (vo, held)):
+            if t.shape != want or t.device != device or not t.is_contiguous():
                 raise ValueError(f"cache tensors must be contiguous, on one device and of matching shapes: got {tuple(t.shape)} on {t.device}, "
-                                 f"expected {shape} on {kc.device}")
-        if ks.dtype != torch.float32 or self.v_scale.dtype != torch.float32:
-            raise ValueError("cache scales are float32")
-
-    lists = property(lambda self: self.k_codes.shape[0])
-    heads = property(lambda self: self.k_codes.shape[1])
-    capacity = property(lambda self: self.k_codes.shape[2] * BLOCK)
-    head_dim = property(lambda self: self.k_open.shape[4])
-    device = property(lambda self: self.k_codes.device)
-    dtype = property(lambda self: self.k_codes.dtype)
+                                 f"expected {tuple(want)} on {device}")
+        # (plain attributes: every call of every op looks them up)
+        self.__dict__.update(lists=L, heads=H, blocks=nb, units=U, capacity=nb * BLOCK, head_dim=D, device=device, dtype=code, open_dtype=kind)
 
 
 def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None, dtype: torch.dtype = torch.int8,
@@ -96,18 +94,21 @@ def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None,
 
 # ----------------------------------------------------------------------------- argument checks (both bodies)
 def check_index(t: Tensor, n: int, name: str, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def check_no_grad(op: str, *tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op} is a decoding op without a backward pass: call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{op} is a decoding op without a backward pass: call it under torch.no_grad()")
 
 
 def check_rows(op: str, t: Tensor, name: str, cache: KV8Cache) -> None:
-    if t.dim() != 3 or t.shape[1] != cache.heads or t.shape[2] != cache.head_dim or t.dtype != cache.k_open.dtype or t.device != cache.device:
-        raise ValueError(f"{op}: {name} must be [rows, {cache.heads}, {cache.head_dim}] {cache.k_open.dtype} on {cache.device}, got "
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != cache.heads or shape[2] != cache.head_dim or t.dtype != cache.open_dtype or t.device != cache.device:
+        raise ValueError(f"{op}: {name} must be [rows, {cache.heads}, {cache.head_dim}] {cache.open_dtype} on {cache.device}, got "
                          f"{tuple(t.shape)} {t.dtype} on {t.device}")
 
 
@@ -134,7 +135,8 @@ def check_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dty
 
 def check_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor, scale: float, max_rows: int, out: Tensor | None) -> None:
     check_no_grad("kv8_attention", q)
-    if (q.dim() != 3 or q.shape[2] != cache.head_dim or q.shape[1] < 1 or q.shape[1] % cache.heads or q.dtype not in FLOATS
+    shape = q.shape
+    if (len(shape) != 3 or shape[2] != cache.head_dim or shape[1] < 1 or shape[1] % cache.heads or q.dtype not in FLOATS
             or q.device != cache.device):
         raise ValueError(f"kv8_attention: q must be [rows, a multiple of {cache.heads}, {cache.head_dim}] bfloat16, float16 or float32 on "
                          f"{cache.device}, got {tuple(q.shape)} {q.dtype} on {q.device}")

@@ -68,6 +68,7 @@ def attention64(q, cache, seg, lengths, scale):
     tol = torch.zeros(q.shape, dtype=torch.float64)
     group = q.shape[1] // cache.heads
     half = torch.finfo(q.dtype).eps / 2
+    lift = 128.0 if q.dtype != torch.float32 and cache.dtype == torch.int8 else 0.0
     for l, length in enumerate(lengths):
         n = int(seg[l + 1] - seg[l])
         for a in range(n):
@@ -77,14 +78,15 @@ def attention64(q, cache, seg, lengths, scale):
             k, v = (values64(cache, w, l, length)[:, :see].repeat_interleave(group, 0) for w in ("k", "v"))
             x = q[int(seg[l]) + a].double().unsqueeze(1)
             s = (x * k).sum(-1) * scale
-            big = ((x * k).abs().sum(-1) * scale).amax(-1)
+            extra = [(lift * t[l].double()).repeat_interleave(64, 1)[:, :see].repeat_interleave(group, 0) for t in (cache.k_scale, cache.v_scale)]
+            big = ((x.abs() * (k.abs() + extra[0].unsqueeze(-1))).sum(-1) * scale).amax(-1)
             p = torch.softmax(s, -1)
             o = (p.unsqueeze(-1) * v).sum(1)
             e = big * (q.shape[2] + 8) * 2.0 ** -23 + 2.0 ** -22 + 2 * s.abs().amax(-1) * 1.45 * 2.0 ** -23
             e = torch.expm1(2 * e) + (2.0 ** -21 if q.dtype == torch.float32 else 2.0 ** -11)
             vmax = v.abs().amax(dim=(1, 2))
             out[int(seg[l]) + a] = o
-            tol[int(seg[l]) + a] = ((2 * e + (see / 16 + 16) * 2.0 ** -23) * vmax).unsqueeze(-1) + half * o.abs() * 1.01
+            tol[int(seg[l]) + a] = (2 * e * vmax + (see / 16 + 16) * 2.0 ** -23 * (vmax + extra[1].amax(-1))).unsqueeze(-1) + half * o.abs() * 1.01
     return out, tol
 
 
