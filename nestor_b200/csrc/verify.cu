@@ -9,9 +9,9 @@
 // Sums are in 64 bits: the running sum has as many steps as the vocabulary has tokens, and a sum in 32 bits would move
 // one draw in some fifty across a step. Values below 2^-126 count as zero.
 //
-// What bounds it: one or two rows of the vocabulary for each sequence, read once from HBM (a few KB are read again to
-// find the token). A row is spread over a cluster of up to 8 CTAs, which exchange their sums through distributed shared
-// memory: one launch, no workspace, a fixed order of additions.
+// What bounds it: one or two rows of the vocabulary for each sequence, read once from HBM (some KB are read again to find
+// the token). A row is cut into spans of 512 entries or more, one warp sums a span, and a cluster of up to 8 CTAs shares a
+// row and exchanges the spans' sums through distributed shared memory: one launch, no workspace, a fixed order of additions.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -23,7 +23,8 @@
 namespace nbv {
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kMaxSpans = 1024;      // spans of a row: their sums (8 KB) stand in every CTA's shared memory
 
 __device__ __forceinline__ float val(const float* p, long i) { return __ldg(p + i); }
 __device__ __forceinline__ float val(const __half* p, long i) { return __half2float(p[i]); }
@@ -45,94 +46,112 @@ __device__ __forceinline__ float weight(const T* p, const T* q, long skip, int j
 template <typename T, int MODE>
 __device__ __forceinline__ double span_sum(const T* p, const T* q, long skip, int a, int b) {
   const int lane = threadIdx.x & 31;
-  double s = 0.;
+  double s0 = 0., s1 = 0.;
   int j = a + lane;
   for (; j + 7 * 32 < b; j += 8 * 32) {
     float w[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = weight<T, MODE>(p, q, skip, j + 32 * i);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += double(w[i]);
+    for (int i = 0; i < 8; i += 2) {
+      s0 += double(w[i]);
+      s1 += double(w[i + 1]);
+    }
   }
-  for (; j < b; j += 32) s += double(weight<T, MODE>(p, q, skip, j));
+  for (; j < b; j += 32) s0 += double(weight<T, MODE>(p, q, skip, j));
+  s0 += s1;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  return s;
+  for (int d = 16; d > 0; d >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, d);
+  return s0;
 }
 
 // The first entry of [a, b) at which `before` plus the running sum passes `goal`; the last one that weighs anything
-// where rounding leaves none.
+// where rounding leaves none. Eight rows of 32 entries at a time: their loads and their scans overlap.
 template <typename T, int MODE>
 __device__ __forceinline__ int find_entry(const T* p, const T* q, long skip, int a, int b, double before, double goal) {
   const int lane = threadIdx.x & 31;
   int last = -1;
-  for (int j0 = a; j0 < b; j0 += 32) {
-    const int j = j0 + lane;
-    const float w = j < b ? weight<T, MODE>(p, q, skip, j) : 0.f;
-    double s = w;
+  for (int j0 = a; j0 < b; j0 += 256) {
+    float w[8];
+    double s[8];
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const double up = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += up;
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + 32 * i + lane;
+      w[i] = j < b ? weight<T, MODE>(p, q, skip, j) : 0.f;
+      s[i] = w[i];
     }
-    const unsigned has = __ballot_sync(0xffffffffu, w > 0.f);
-    const unsigned hit = __ballot_sync(0xffffffffu, w > 0.f && before + s > goal);
-    if (hit) return j0 + __ffs(hit) - 1;
-    if (has) last = j0 + 31 - __clz(has);
-    before += __shfl_sync(0xffffffffu, s, 31);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double up = __shfl_up_sync(0xffffffffu, s[i], d);
+        if (lane >= d) s[i] += up;
+      }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const unsigned has = __ballot_sync(0xffffffffu, w[i] > 0.f);
+      const unsigned hit = __ballot_sync(0xffffffffu, w[i] > 0.f && before + s[i] > goal);
+      if (hit) return j0 + 32 * i + __ffs(hit) - 1;
+      if (has) last = j0 + 32 * i + 31 - __clz(has);
+      before += __shfl_sync(0xffffffffu, s[i], 31);
+    }
   }
   return last;
 }
 
-// Draws from the row; returns false if nothing weighs anything. All CTAs of the cluster call it together.
+// Draws from the row; returns false if nothing weighs anything. All CTAs of the cluster call it together. Span i belongs
+// to warp i % (warps of the cluster); a CTA keeps the sums of its spans at their places in `all` and copies the others'.
 template <typename T, int MODE>
-__device__ __forceinline__ bool draw(const nb_verify_args& a, const T* p, const T* q, long skip, float w, int b, double* sums, double* all) {
+__device__ __forceinline__ bool draw(const nb_verify_args& a, int span, const T* p, const T* q, long skip, float w, int b, double* all) {
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = a.V;
-  const int spans = CL * kWarps, per = (V + spans - 1) / spans;
-  const int mine = rank * kWarps + warp, lo = min(V, mine * per), hi = min(V, lo + per);
-  const double s = span_sum<T, MODE>(p, q, skip, lo, hi);
-  if (lane == 0) sums[warp] = s;
-  cluster.sync();
-  if (threadIdx.x < spans) all[threadIdx.x] = cluster.map_shared_rank(sums, threadIdx.x / kWarps)[threadIdx.x % kWarps];
-  __syncthreads();
-  // running sums over the spans, the same in every warp: lane by lane over 4 spans each
-  double part[4], run = 0.;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int at = lane * 4 + i;
-    run += at < spans ? all[at] : 0.;
-    part[i] = run;
+  const int spans = (V + span - 1) / span, step = CL * kWarps;
+  for (int i = rank * kWarps + warp; i < spans; i += step) {
+    const double s = span_sum<T, MODE>(p, q, skip, i * span, min(V, (i + 1) * span));
+    if (lane == 0) all[i] = s;
   }
+  cluster.sync();
+  for (int i = threadIdx.x; i < spans; i += kThreads) {
+    const int owner = i % step / kWarps;
+    if (owner != rank) all[i] = cluster.map_shared_rank(all, owner)[i];
+  }
+  __syncthreads();
+  // running sums over the spans, the same in every warp: each lane over `per` consecutive ones
+  const int per = (spans + 31) / 32, first = min(spans, lane * per), end = min(spans, first + per);
+  double run = 0.;
+  for (int i = first; i < end; ++i) run += all[i];
   double incl = run;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
     const double up = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += up;
   }
-  const double total = __shfl_sync(0xffffffffu, incl, 31), before = incl - run, goal = double(w) * total;
+  const double goal = double(w) * __shfl_sync(0xffffffffu, incl, 31);
   // the first span whose running sum passes the goal; failing that the last one that weighs anything
-  int first = 1 << 20, last = -1;
-#pragma unroll
-  for (int i = 3; i >= 0; --i) {
-    const int at = lane * 4 + i;
-    if (at < spans && all[at] > 0.) {
-      if (before + part[i] > goal) first = at;
-      last = max(last, at);
+  int hit = kMaxSpans, last = -1;
+  double before = incl - run, ahead = 0.;
+  for (int i = first; i < end; ++i) {
+    const double s = all[i];
+    if (s > 0.) {
+      if (hit == kMaxSpans && before + s > goal) {
+        hit = i;
+        ahead = before;
+      }
+      last = i;
+      if (hit == kMaxSpans) ahead = before;
     }
+    before += s;
   }
-  first = __reduce_min_sync(0xffffffffu, first);
-  last = __reduce_max_sync(0xffffffffu, last);
-  const int span = first < spans ? first : last;
-  if (span < 0) {
+  const int hit_all = __reduce_min_sync(0xffffffffu, hit), last_all = __reduce_max_sync(0xffffffffu, last);
+  const int at = hit_all < kMaxSpans ? hit_all : last_all;
+  if (at < 0) {
     cluster.sync();      // (the sums are written again by the next draw)
     return false;
   }
-  if (span == mine) {
-    double ahead = 0.;
-    for (int i = 0; i < span; ++i) ahead += all[i];
-    const int j = find_entry<T, MODE>(p, q, skip, lo, hi, ahead, goal);
+  if (at % step == rank * kWarps + warp) {
+    ahead = __shfl_sync(0xffffffffu, ahead, at / per);
+    const int j = find_entry<T, MODE>(p, q, skip, at * span, min(V, (at + 1) * span), ahead, goal);
     if (lane == 0) a.token[b] = j;
   }
   cluster.sync();        // no CTA leaves while another may read its sums
@@ -140,8 +159,8 @@ __device__ __forceinline__ bool draw(const nb_verify_args& a, const T* p, const 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const nb_verify_args a) {
-  __shared__ double sums[kWarps], all[kMaxCluster * kWarps];
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const nb_verify_args a, int span) {
+  __shared__ double all[kMaxSpans];
   cg::cluster_group cluster = cg::this_cluster();
   const int b = blockIdx.x / cluster.num_blocks(), lane = threadIdx.x & 31;
   const T* P = reinterpret_cast<const T*>(a.p) + long(b) * a.p_batch;
@@ -172,10 +191,10 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const nb_verify_args a
   const T* p = P + accepted * a.p_row;
   const float w = a.w[b];
   bool done;
-  if (accepted == len) done = draw<T, 0>(a, p, nullptr, -1, w, b, sums, all);
+  if (accepted == len) done = draw<T, 0>(a, span, p, nullptr, -1, w, b, all);
   else {
-    done = Q ? draw<T, 1>(a, p, Q + accepted * a.q_row, -1, w, b, sums, all) : draw<T, 2>(a, p, nullptr, token(accepted), w, b, sums, all);
-    if (!done) done = draw<T, 0>(a, p, nullptr, -1, w, b, sums, all);
+    done = Q ? draw<T, 1>(a, span, p, Q + accepted * a.q_row, -1, w, b, all) : draw<T, 2>(a, span, p, nullptr, token(accepted), w, b, all);
+    if (!done) done = draw<T, 0>(a, span, p, nullptr, -1, w, b, all);
   }
   if (cluster.block_rank() == 0 && threadIdx.x == 0) {
     a.accepted[b] = accepted;
@@ -187,11 +206,16 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const nb_verify_args a
 
 extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
   using namespace nbv;
-  if (a->B < 0 || a->n < 0 || a->V < 1 || a->type < 0 || a->type > 2) return -1;
+  if (a->B < 0 || a->n < 0 || a->V < 1 || a->V > (1 << 30) || a->type < 0 || a->type > 2) return -1;
   if (a->B == 0) return 0;
-  // a CTA for each 4096 entries: fewer would leave warps without work, and one CTA reads so many in a microsecond
+  // spans that keep the sums within their 8 KB, and no more CTAs a row than there are spans for half of their warps or than
+  // fit the GPU at once (4 an SM): a second wave would wait for its first loads while the first one's end idles
+  int span = 512;
+  while ((a->V + span - 1) / span > kMaxSpans) span *= 2;
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   int cl = 1;
-  while (cl < kMaxCluster && cl * 4096 < a->V) cl *= 2;
+  while (cl < kMaxCluster && cl * kWarps * span < 2 * a->V && long(a->B) * cl * 2 <= 4l * sms) cl *= 2;
   if (long(a->B) * cl > 0x7fffffffl) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a->B) * cl);
@@ -203,9 +227,9 @@ extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t rc = a->type == 0   ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16>, *a)
-                   : a->type == 1 ? cudaLaunchKernelEx(&cfg, verify_kernel<__half>, *a)
-                                  : cudaLaunchKernelEx(&cfg, verify_kernel<float>, *a);
+  cudaError_t rc = a->type == 0   ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16>, *a, span)
+                   : a->type == 1 ? cudaLaunchKernelEx(&cfg, verify_kernel<__half>, *a, span)
+                                  : cudaLaunchKernelEx(&cfg, verify_kernel<float>, *a, span);
   if (rc != cudaSuccess) return int(rc);
   return int(cudaGetLastError());
 }

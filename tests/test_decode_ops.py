@@ -618,7 +618,7 @@ def test_decode_step_in_graphs_and_on_streams():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("kind", TYPES)
-@pytest.mark.parametrize("V", [1, 5, 1000, 4097, 50257, 100263])
+@pytest.mark.parametrize("V", [1, 5, 1000, 4097, 50257, 100263, 700001])
 def test_verification_kernel(kind, V):
     for n, greedy in ((0, False), (4, False), (3, True), (40, False)):
         if n == 40 and V > 5000:
