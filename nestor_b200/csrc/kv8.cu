@@ -55,88 +55,180 @@ template <> __device__ __forceinline__ float from_f(float x) { return x; }
 template <> __device__ __forceinline__ __half from_f(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T x[VEC]; };
-
-// Entry and dim of byte b (0..15) of lane (g, t) in unit u.
-__device__ __forceinline__ int unit_entry(int kv, int g, int t, int b) {
-  return ((b >> 2) << 4) + (((b >> 1) & 1) << 3) + (kv ? 2 * t + (b & 1) : g);
-}
-__device__ __forceinline__ int unit_dim(int kv, int g, int t, int b) { return kv ? g : 2 * t + (b & 1); }
-
 // ------------------------------------------------------------------------------------------------------- append
-// One CTA stores one block of one head of the keys or the values: entries [0, t0) come from the originals that the
-// cache keeps (`open`), entries [t0, t0 + m) are new rows. The block's largest magnitude (compared as integers, so that
-// a NaN counts as the largest) gives scale = amax / Q and code = round_half_even(x * (Q / amax)), Q = 127 or 448.
-// A block with an infinity or a NaN takes the scale NaN: all its values are NaN. A block below 2^-100 holds zeros.
-template <typename T, int VEC, int CODE>
-__device__ __forceinline__ void store_block(const nb_kv8_cache& c, int kv, long lh, int b, int t0, int m,
-                                            const T* __restrict__ src, long row_stride, float* tile, unsigned* red) {
-  const int D = c.D, pitch = D | 1, nv = D / VEC, T_tok = t0 + m;
-  const T* held = reinterpret_cast<const T*>(c.open[kv]) + ((lh * 2 + (b & 1)) * kBlock) * long(D);
-  unsigned top = 0;
-  for (int i = threadIdx.x; i < T_tok * nv; i += blockDim.x) {
-    const int e = i / nv, j = (i - e * nv) * VEC;
-    const T* from = e < t0 ? held + long(e) * D + j : src + long(e - t0) * row_stride + j;
-    const Vec<T, VEC> v = *reinterpret_cast<const Vec<T, VEC>*>(from);
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) {
-      const float f = to_f(v.x[q]);
-      top = max(top, __float_as_uint(f) & 0x7fffffffu);
-      tile[e * pitch + j + q] = f;
-    }
-  }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-  __syncthreads();
-  for (int w = 0; w < int(blockDim.x >> 5); ++w) top = max(top, red[w]);
-  constexpr float Q = CODE == 0 ? 127.f : 448.f;
-  const float amax = __uint_as_float(top);
-  const bool poison = top >= 0x7f800000u, empty = amax < 0x1p-100f;
-  const float fit = poison || empty ? 0.f : __fdiv_rn(Q, amax);
-  const float scale = poison ? __uint_as_float(0x7fc00000u) : (empty ? 0.f : __fdiv_rn(amax, Q));
-  uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.codes[kv]) + (lh * c.nb + b) * (long(c.U) * 512));
-  for (int i = threadIdx.x; i < c.U * 32; i += blockDim.x) {
-    const int u = i >> 5, g = (i >> 2) & 7, t = i & 3;
-    unsigned word[4];
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float y[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int e = unit_entry(kv, g, t, 4 * w + q), d = 8 * u + unit_dim(kv, g, t, 4 * w + q);
-        y[q] = fit != 0.f && e < T_tok && d < D ? __fmul_rn(tile[e * pitch + d], fit) : 0.f;
-      }
-      if constexpr (CODE == 0) {
-        // adding 1.5 * 2^23 leaves the integer, rounded half to even, in the low bits; |y| <= 127 (1 + 2^-23)
-        unsigned r[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) r[q] = __float_as_uint(__fadd_rn(y[q], 12582912.f)) & 0xffu;
-        word[w] = r[0] | (r[1] << 8) | (r[2] << 16) | (r[3] << 24);
-      } else {
-        const unsigned a = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
-        const unsigned z = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
-        word[w] = a | (z << 16);
-      }
-    }
-    out[i] = make_uint4(word[0], word[1], word[2], word[3]);
-  }
-  if (threadIdx.x == 0) c.scale[kv][lh * c.nb + b] = scale;
+// One CTA stores a block of one head, keys and values: entries [0, t0) come from the originals that the cache keeps
+// (`open`), entries [t0, t0 + m) are new rows. The block's largest magnitude gives scale = amax / Q and
+// code = round_half_even(x * (Q / amax)), Q = 127 or 448. A block with an infinity or a NaN takes the scale NaN: all its
+// values are NaN. A block below 2^-100 holds zeros.
+//
+// A warp owns a unit (two of them above 8): its lanes load the pairs of dims of eight entries that they hold in the keys'
+// layout, so nothing passes through shared memory but the warps' maxima. The values' layout is the transpose of each
+// 8 x 8 tile: their codes go through movmatrix as 16-bit numbers. About 6 instructions an element; through a tile in
+// shared memory it was 20, and those, not HBM, were the bound.
+__device__ __forceinline__ unsigned transpose8x8(unsigned x) {
+  unsigned y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {      // (a NaN stays)
+  float c;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+  return c;
 }
 
-// grid (ceil(rows / chunk), H, 2). A CTA looks through its chunk of rows for those that begin a block or a list and
-// stores the block that each of them begins; the others exit. `chunk` is 1 for steps of few rows a list (every row may
-// begin a block: one CTA each) and 64 for prompts (one block a CTA). The CTA of a list's first row also files the
-// originals of the new rows of the youngest two blocks: it alone reads the older originals, so nothing races with it.
-template <typename T, int VEC, int CODE>
-__global__ void __launch_bounds__(128) append_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
-  extern __shared__ float tile[];
-  __shared__ unsigned red[4];
-  const int kv = blockIdx.z, h = blockIdx.y, cap = c.nb * kBlock;
+// Two neighbouring elements as they stand in memory (one register for 16-bit types). PAIR: as one access of that size.
+template <typename T> struct Raw { using type = unsigned; };
+template <> struct Raw<float> { using type = float2; };
+template <typename T> using Two = typename Raw<T>::type;
+
+__device__ __forceinline__ float2 floats(unsigned v, __nv_bfloat16) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+__device__ __forceinline__ float2 floats(unsigned v, __half) { return __half22float2(reinterpret_cast<const __half2&>(v)); }
+__device__ __forceinline__ float2 floats(float2 v, float) { return v; }
+__device__ __forceinline__ void make_zero(unsigned& v) { v = 0u; }
+__device__ __forceinline__ void make_zero(float2& v) { v = make_float2(0.f, 0.f); }
+
+template <typename T, bool PAIR>
+__device__ __forceinline__ Two<T> load_two(const T* p, bool second) {
+  if constexpr (PAIR) return *reinterpret_cast<const Two<T>*>(p);
+  if constexpr (sizeof(T) == 4) return make_float2(p[0], second ? p[1] : 0.f);
+  else {
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    return unsigned(h[0]) | (second ? unsigned(h[1]) << 16 : 0u);
+  }
+}
+template <typename T, bool PAIR>
+__device__ __forceinline__ void store_two(T* p, Two<T> v, bool second) {
+  if constexpr (PAIR) *reinterpret_cast<Two<T>*>(p) = v;
+  else if constexpr (sizeof(T) == 4) {
+    p[0] = v.x;
+    if (second) p[1] = v.y;
+  } else {
+    unsigned short* h = reinterpret_cast<unsigned short*>(p);
+    h[0] = static_cast<unsigned short>(v & 0xffffu);
+    if (second) h[1] = static_cast<unsigned short>(v >> 16);
+  }
+}
+__device__ __forceinline__ unsigned rounded(float2 y, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(y.x, y.y);
+  return reinterpret_cast<const unsigned&>(v);
+}
+__device__ __forceinline__ unsigned rounded(float2 y, __half) {
+  const __half2 v = __floats2half2_rn(y.x, y.y);
+  return reinterpret_cast<const unsigned&>(v);
+}
+__device__ __forceinline__ float2 rounded(float2 y, float) { return y; }
+
+template <int CODE>
+__device__ __forceinline__ unsigned code_pair(float2 y) {          // codes of y.x and y.y in bits 0..7 and 8..15
+  if constexpr (CODE == 0)
+    // adding 1.5 * 2^23 leaves the integer, rounded half to even, in the low bits; |y| <= 127 (1 + 2^-23)
+    return __byte_perm(__float_as_uint(__fadd_rn(y.x, 12582912.f)), __float_as_uint(__fadd_rn(y.y, 12582912.f)), 0x0040) & 0xffffu;
+  else
+    return __nv_cvt_float2_to_fp8x2(y, __NV_SATFINITE, __NV_E4M3);
+}
+
+struct Source {            // where a block's entries are: the first t0 in `held`, the next m in `rows`
+  const void *held, *rows;
+  long row_stride;
+};
+
+template <typename T, bool PAIR, int CODE, int NU>
+__device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int b, int t0, int m, const Source (&src)[2], bool keep, float (*red)[8]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3, D = c.D, n = t0 + m;
+  // (entries and dims that are not there load one that is, so that all loads are in flight at once, and become zeros)
+  Two<T> x[2][NU][8];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = min(8 * i + g, n - 1);
+      const T* from = e < t0 ? reinterpret_cast<const T*>(src[kv].held) + e * D : reinterpret_cast<const T*>(src[kv].rows) + (e - t0) * src[kv].row_stride;
+#pragma unroll
+      for (int a = 0; a < NU; ++a) {
+        const int d = 8 * (warp + a * warps) + 2 * t;
+        x[kv][a][i] = load_two<T, PAIR>(from + (d < D ? d : 0), d + 1 < D);
+      }
+    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int a = 0; a < NU; ++a)
+      if (8 * i + g >= n || 8 * (warp + a * warps) + 2 * t >= D)
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) make_zero(x[kv][a][i]);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float top = 0.f;
+#pragma unroll
+    for (int a = 0; a < NU; ++a)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 y = floats(x[kv][a][i], T{});
+        top = max_nan(top, max_nan(fabsf(y.x), fabsf(y.y)));
+      }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, s));
+    if (lane == 0) red[kv][warp] = top;
+  }
+  __syncthreads();      // (behind it no thread has an older original left to load)
+  if (keep) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int a = 0; a < NU; ++a) {
+        const int e = 8 * i + g, d = 8 * (warp + a * warps) + 2 * t;
+        if (e >= t0 && e < n && d < D)
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            T* to = reinterpret_cast<T*>(c.open[kv]) + ((lh * 2 + (b & 1)) * kBlock + e) * D + d;
+            store_two<T, PAIR>(to, x[kv][a][i], d + 1 < D);
+          }
+      }
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    float amax = red[kv][0];
+    for (int w = 1; w < warps; ++w) amax = max_nan(amax, red[kv][w]);
+    constexpr float Q = CODE == 0 ? 127.f : 448.f;
+    const bool poison = !(amax < INFINITY), empty = amax < 0x1p-100f;
+    const float fit = poison || empty ? 0.f : __fdiv_rn(Q, amax);
+    uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.codes[kv]) + (lh * c.nb + b) * (long(c.U) * 512)) + lane;
+    if (threadIdx.x == 0)
+      c.scale[kv][lh * c.nb + b] = poison ? __uint_as_float(0x7fc00000u) : (empty ? 0.f : __fdiv_rn(amax, Q));
+#pragma unroll
+    for (int a = 0; a < NU; ++a) {
+      const int u = warp + a * warps;
+      unsigned word[4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        unsigned half[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 v = floats(x[kv][a][2 * w + i], T{});
+          // (zero times a poisoned block's NaN is a NaN: its codes are made zero)
+          half[i] = code_pair<CODE>(poison ? make_float2(0.f, 0.f) : make_float2(__fmul_rn(v.x, fit), __fmul_rn(v.y, fit)));
+          if (kv == 1) half[i] = transpose8x8(__byte_perm(half[i], 0u, 0x4140));
+        }
+        word[w] = __byte_perm(half[0], half[1], kv == 0 ? 0x5410 : 0x6420);
+      }
+      if (u < c.U) out[u * 32] = make_uint4(word[0], word[1], word[2], word[3]);
+    }
+  }
+}
+
+// grid (ceil(rows / chunk), H), a warp for each unit or two. A CTA looks through its chunk of rows for those that begin a
+// block or a list and stores the block that each of them begins; the others exit. The two youngest blocks' new rows are
+// kept as originals, by the CTA that stores the block. One case is different: an append that begins inside a block b0
+// and goes on to b0 + 2 and further. Those blocks take the slot from which b0's older originals are read, so the CTA of
+// the list's first row files their rows itself, after it has read them.
+template <typename T, bool PAIR, int CODE, int NU>
+__global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) append_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
+  __shared__ float red[2][2][8];
+  const int h = blockIdx.y, cap = c.nb * kBlock, D = c.D;
   const int end = min(p.seg[c.L], p.rows);
-  int r = blockIdx.x * chunk;
+  int r = blockIdx.x * chunk, turn = 0;
   const int r1 = min(r + chunk, end);
-  const long rs = p.row_stride[kv];
-  const T* rows = reinterpret_cast<const T*>(p.src[kv]) + h * p.head_stride[kv];
+  const T* rows[2] = {reinterpret_cast<const T*>(p.src[0]) + h * p.head_stride[0], reinterpret_cast<const T*>(p.src[1]) + h * p.head_stride[1]};
   while (r < r1) {
     const int l = find_list(p.seg, c.L, r);
     const int s0 = p.seg[l], s1 = p.seg[l + 1], at = p.start[l];
@@ -151,17 +243,27 @@ __global__ void __launch_bounds__(128) append_kernel(nb_kv8_cache c, nb_kv8_rows
     }
     const long lh = long(l) * c.H + h;
     while (r < s1 && r < r1) {
-      const int e = at + (r - s0), t = e & (kBlock - 1), m = min(kBlock - t, s1 - r);
+      const int e = at + (r - s0), b = e / kBlock, t = e & (kBlock - 1), m = min(kBlock - t, s1 - r);
       if (r == s0 || t == 0) {
-        store_block<T, VEC, CODE>(c, kv, lh, e / kBlock, t, m, rows + long(r) * rs, rs, tile, red);
-        __syncthreads();
-        if (r == s0) {
-          const int last = (at + (s1 - s0) - 1) / kBlock, from = max(at, (last - 1) * kBlock), nv = c.D / VEC;
-          T* held = reinterpret_cast<T*>(c.open[kv]) + lh * 2 * kBlock * long(c.D);
-          for (int i = threadIdx.x; i < (at + (s1 - s0) - from) * nv; i += blockDim.x) {
-            const int q = i / nv, j = (i - q * nv) * VEC, to = from + q;
-            *reinterpret_cast<Vec<T, VEC>*>(held + ((to / kBlock & 1) * kBlock + (to & (kBlock - 1))) * long(c.D) + j) =
-                *reinterpret_cast<const Vec<T, VEC>*>(rows + long(s0 + to - at) * rs + j);
+        Source src[2];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          src[kv].held = reinterpret_cast<const T*>(c.open[kv]) + (lh * 2 + (b & 1)) * kBlock * long(D);
+          src[kv].rows = rows[kv] + long(r) * p.row_stride[kv];
+          src[kv].row_stride = p.row_stride[kv];
+        }
+        const int b0 = at / kBlock, last = (at + (s1 - s0) - 1) / kBlock;
+        const bool clash = (at & (kBlock - 1)) != 0 && last >= b0 + 2;
+        store_block<T, PAIR, CODE, NU>(c, lh, b, t, m, src, b >= last - 1 && (!clash || b < b0 + 2), red[turn]);
+        turn ^= 1;
+        if (r == s0 && clash) {
+          const int from = max(last - 1, b0 + 2) * kBlock;
+#pragma unroll 4
+          for (int i = threadIdx.x; i < (at + (s1 - s0) - from) * D; i += blockDim.x) {
+            const int q = i / D, d = i - q * D, to = from + q;
+            const long place = (lh * 2 + (to / kBlock & 1)) * kBlock * long(D) + (to & (kBlock - 1)) * D + d;
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) reinterpret_cast<T*>(c.open[kv])[place] = rows[kv][long(s0 + to - at) * p.row_stride[kv] + d];
           }
         }
       }
@@ -170,36 +272,51 @@ __global__ void __launch_bounds__(128) append_kernel(nb_kv8_cache c, nb_kv8_rows
   }
 }
 
-// grid (L, H, 2): re-quantises the partly filled youngest block of every list from its first len % 64 originals.
-template <typename T, int VEC, int CODE>
-__global__ void __launch_bounds__(128) truncate_kernel(nb_kv8_cache c, const int* __restrict__ len) {
-  extern __shared__ float tile[];
-  __shared__ unsigned red[4];
+// grid (L, H): re-quantises the partly filled youngest block of every list from its first len % 64 originals.
+template <typename T, bool PAIR, int CODE, int NU>
+__global__ void __launch_bounds__(256) truncate_kernel(nb_kv8_cache c, const int* __restrict__ len) {
+  __shared__ float red[2][8];
   const int l = blockIdx.x, n = len[l];
   if (n < 0 || n > c.nb * kBlock) {
     if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
     return;
   }
   if ((n & (kBlock - 1)) == 0) return;
-  store_block<T, VEC, CODE>(c, blockIdx.z, long(l) * c.H + blockIdx.y, n / kBlock, n & (kBlock - 1), 0, nullptr, 0, tile, red);
+  const long lh = long(l) * c.H + blockIdx.y;
+  Source src[2];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) src[kv] = {reinterpret_cast<const T*>(c.open[kv]) + (lh * 2 + (n / kBlock & 1)) * kBlock * long(c.D), nullptr, 0};
+  store_block<T, PAIR, CODE, NU>(c, lh, n / kBlock, n & (kBlock - 1), 0, src, false, red);
 }
 
 // --------------------------------------------------------------------------------------------------------- read
-// The inverse of append, with the same division of rows over CTAs; rows behind the last list become zeros.
-template <typename T, int VEC, int CODE>
-__global__ void __launch_bounds__(128) read_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
-  extern __shared__ float tile[];
-  const int kv = blockIdx.z, h = blockIdx.y, cap = c.nb * kBlock, D = c.D, pitch = D | 1, nv = D / VEC;
+template <int CODE>
+__device__ __forceinline__ float2 decoded(unsigned pair) {         // of codes in bits 0..7 and 8..15
+  if constexpr (CODE == 0) {
+    // (128 + x in the low bits of a float with the exponent of 2^23; the subtraction is exact)
+    const unsigned u = pair ^ 0x8080u;
+    return make_float2(__fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440)), 8388736.f),
+                       __fsub_rn(__uint_as_float(__byte_perm(u, 0x4b000000u, 0x7441)), 8388736.f));
+  } else {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(pair), __NV_E4M3);
+    return __half22float2(reinterpret_cast<const __half2&>(h));
+  }
+}
+
+// The inverse of append, with the same division of rows over CTAs and of units over warps; rows behind the last list
+// become zeros.
+template <typename T, bool PAIR, int CODE, int NU>
+__global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
+  const int h = blockIdx.y, cap = c.nb * kBlock, D = c.D;
   const int end = max(0, min(p.seg[c.L], p.rows));
-  T* dst = reinterpret_cast<T*>(p.dst[kv]) + long(h) * D;
+  T* dst[2] = {reinterpret_cast<T*>(p.dst[0]) + long(h) * D, reinterpret_cast<T*>(p.dst[1]) + long(h) * D};
   const long rs = long(c.H) * D;
   auto zeros = [&](int a, int b) {
-    Vec<T, VEC> z;
-#pragma unroll
-    for (int q = 0; q < VEC; ++q) z.x[q] = from_f<T>(0.f);
-    for (int i = threadIdx.x; i < (b - a) * nv; i += blockDim.x) {
-      const int e = i / nv, j = (i - e * nv) * VEC;
-      *reinterpret_cast<Vec<T, VEC>*>(dst + long(a + e) * rs + j) = z;
+    for (int i = threadIdx.x; i < (b - a) * D; i += blockDim.x) {
+      const int e = i / D;
+      const long at = long(a + e) * rs + (i - e * D);
+      dst[0][at] = dst[1][at] = from_f<T>(0.f);
     }
   };
   int r = blockIdx.x * chunk;
@@ -207,13 +324,13 @@ __global__ void __launch_bounds__(128) read_kernel(nb_kv8_cache c, nb_kv8_rows p
   if (r_end > max(r, end)) zeros(max(r, end), r_end);
   while (r < r1) {
     const int l = find_list(p.seg, c.L, r);
-    const int s0 = p.seg[l], s1 = min(p.seg[l + 1], p.rows), at = p.start[l];
+    const int s0 = p.seg[l], s1 = p.seg[l + 1], at = p.start[l];
     if (s0 > r || s1 <= r || s0 < 0) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
       zeros(r, r1);
       return;
     }
-    if (at < 0 || long(at) + (p.seg[l + 1] - s0) > cap || p.seg[l + 1] > end) {
+    if (s1 > end || at < 0 || long(at) + (s1 - s0) > cap) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
       zeros(r, min(s1, r1));
       r = s1;
@@ -223,32 +340,30 @@ __global__ void __launch_bounds__(128) read_kernel(nb_kv8_cache c, nb_kv8_rows p
     while (r < s1 && r < r1) {
       const int e0 = at + (r - s0), t0 = e0 & (kBlock - 1), m = min(kBlock - t0, s1 - r), b = e0 / kBlock;
       if (r == s0 || t0 == 0) {
-        const uint4* in = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.codes[kv]) + (lh * c.nb + b) * (long(c.U) * 512));
-        const float scale = c.scale[kv][lh * c.nb + b];
-        __syncthreads();
-        for (int i = threadIdx.x; i < c.U * 32; i += blockDim.x) {
-          const uint4 w4 = in[i];
-          const unsigned word[4] = {w4.x, w4.y, w4.z, w4.w};
-          const int u = i >> 5, g = (i >> 2) & 7, t = i & 3;
 #pragma unroll
-          for (int w = 0; w < 4; ++w)
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint4* in = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.codes[kv]) + (lh * c.nb + b) * (long(c.U) * 512)) + lane;
+          const float scale = c.scale[kv][lh * c.nb + b];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int e = unit_entry(kv, g, t, 4 * w + q), d = 8 * u + unit_dim(kv, g, t, 4 * w + q);
-              const unsigned byte = (word[w] >> (8 * q)) & 0xffu;
-              float x;
-              if constexpr (CODE == 0) x = float(int8_t(byte));
-              else x = __half2float(__half(__nv_cvt_fp8_to_halfraw(__nv_fp8_storage_t(byte), __NV_E4M3)));
-              if (d < D) tile[e * pitch + d] = __fmul_rn(x, scale);
+          for (int a = 0; a < NU; ++a) {
+            const int u = warp + a * warps, d = 8 * u + 2 * t;
+            const uint4 w4 = u < c.U ? in[u * 32] : make_uint4(0, 0, 0, 0);
+            const unsigned word[4] = {w4.x, w4.y, w4.z, w4.w};
+            unsigned pair[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              pair[i] = (word[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+              if (kv == 1) pair[i] = __byte_perm(transpose8x8(__byte_perm(pair[i], 0u, 0x4140)), 0u, 0x4420);
             }
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < m * nv; i += blockDim.x) {
-          const int e = i / nv, j = (i - e * nv) * VEC;
-          Vec<T, VEC> v;
 #pragma unroll
-          for (int q = 0; q < VEC; ++q) v.x[q] = from_f<T>(tile[(t0 + e) * pitch + j + q]);
-          *reinterpret_cast<Vec<T, VEC>*>(dst + long(r + e) * rs + j) = v;
+            for (int i = 0; i < 8; ++i) {
+              const int e = 8 * i + g - t0;
+              if (e >= 0 && e < m && d < D) {
+                const float2 y = decoded<CODE>(pair[i]);
+                store_two<T, PAIR>(dst[kv] + long(r + e) * rs + d, rounded(make_float2(__fmul_rn(y.x, scale), __fmul_rn(y.y, scale)), T{}), d + 1 < D);
+              }
+            }
+          }
         }
       }
       r += m;
@@ -321,11 +436,6 @@ __device__ __forceinline__ void mma(float (&d)[4], unsigned a0, unsigned a1, uns
 __device__ __forceinline__ void mma_from(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0, unsigned b1, float c0, float c1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ unsigned transpose8x8(unsigned x) {
-  unsigned y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
 }
 __device__ __forceinline__ unsigned pack(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -1013,33 +1123,40 @@ long slot_floats(int U, int cols) { return long(cols) * (8 * U + 2); }
 long workers_of(int U, int nt) { return long(multiprocessors()) * warps_of(width_of(U), nt); }
 
 
-// The widest vector (at most 16 bytes) that divides the head and that every row start is aligned to.
-int vector_of(int D, int size, const long* strides, int n_strides, const void* const* ptrs, int n_ptrs) {
-  for (int v = 16 / size; v > 1; v >>= 1) {
-    bool ok = D % v == 0;
-    for (int i = 0; i < n_strides; ++i) ok = ok && strides[i] % v == 0;
-    for (int i = 0; i < n_ptrs; ++i) ok = ok && (reinterpret_cast<uintptr_t>(ptrs[i]) % (v * size)) == 0;
-    if (ok) return v;
-  }
-  return 1;
+// Whether every pair of dims (2i, 2i + 1) of every row is aligned to the pair's size.
+bool pairs(int D, int size, const long* strides, int n_strides, const void* const* ptrs, int n_ptrs) {
+  bool ok = D % 2 == 0;
+  for (int i = 0; i < n_strides; ++i) ok = ok && strides[i] % 2 == 0;
+  for (int i = 0; i < n_ptrs; ++i) ok = ok && reinterpret_cast<uintptr_t>(ptrs[i]) % (2 * size) == 0;
+  return ok;
 }
 
-// f(type tag, vector tag, code tag) for the run-time triple
+// f(type tag, pair tag, code tag, units-a-warp tag) for the run-time values
 template <typename F>
-void with_types(int type, int vec, int code, F f) {
+void with_types(int type, bool pair, int code, int U, F f) {
+  auto by_units = [&](auto t, auto v, auto k) {
+    if (U <= 8) f(t, v, k, std::integral_constant<int, 1>{});
+    else f(t, v, k, std::integral_constant<int, 2>{});
+  };
   auto by_code = [&](auto t, auto v) {
-    if (code == 0) f(t, v, std::integral_constant<int, 0>{});
-    else f(t, v, std::integral_constant<int, 1>{});
+    if (code == 0) by_units(t, v, std::integral_constant<int, 0>{});
+    else by_units(t, v, std::integral_constant<int, 1>{});
   };
-  auto by_vec = [&](auto t) {
-    if (vec == 8 && sizeof(t) == 2) by_code(t, std::integral_constant<int, 8>{});
-    else if (vec == 4) by_code(t, std::integral_constant<int, 4>{});
-    else if (vec == 2) by_code(t, std::integral_constant<int, 2>{});
-    else by_code(t, std::integral_constant<int, 1>{});
+  auto by_pair = [&](auto t) {
+    if (pair) by_code(t, std::true_type{});
+    else by_code(t, std::false_type{});
   };
-  if (type == 0) by_vec(__nv_bfloat16{});
-  else if (type == 1) by_vec(__half{});
-  else by_vec(float{});
+  if (type == 0) by_pair(__nv_bfloat16{});
+  else if (type == 1) by_pair(__half{});
+  else by_pair(float{});
+}
+int unit_threads(int U) { return 32 * (U <= 8 ? U : (U + 1) / 2); }
+
+// Rows that one CTA looks through. Steps of few rows a list: one, since every row may begin a block. Longer runs: a block
+// each, or four where that still leaves two waves of CTAs (the search for the list and the first load are then paid once).
+int chunk_of(int rows, int max_rows, int heads) {
+  if (max_rows <= 8) return 1;
+  return long(rows) * heads / (4 * kBlock) >= 2l * 12 * multiprocessors() ? 4 * kBlock : kBlock;
 }
 
 bool bad_cache(const nb_kv8_cache* c) {
@@ -1054,15 +1171,13 @@ int nb_kv8_append(const nb_kv8_cache* c, const nb_kv8_rows* p, cudaStream_t st) 
   using namespace nbk;
   if (bad_cache(c) || p->rows < 0) return -1;
   if (p->rows == 0) return 0;
-  const int size = c->type == 2 ? 4 : 2;
   const long strides[4] = {p->row_stride[0], p->row_stride[1], p->head_stride[0], p->head_stride[1]};
   const void* ptrs[4] = {p->src[0], p->src[1], c->open[0], c->open[1]};
-  const int vec = vector_of(c->D, size, strides, 4, ptrs, 4);
-  const int chunk = p->max_rows <= 8 ? 1 : kBlock;
-  const dim3 grid((p->rows + chunk - 1) / chunk, c->H, 2);
-  const size_t smem = kBlock * (c->D | 1) * sizeof(float);
-  with_types(c->type, vec, c->code, [&](auto t, auto v, auto k) {
-    append_kernel<decltype(t), decltype(v)::value, decltype(k)::value><<<grid, 128, smem, st>>>(*c, *p, chunk);
+  const bool pair = pairs(c->D, c->type == 2 ? 4 : 2, strides, 4, ptrs, 4);
+  const int chunk = chunk_of(p->rows, p->max_rows, c->H);
+  const dim3 grid((p->rows + chunk - 1) / chunk, c->H);
+  with_types(c->type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
+    append_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<grid, unit_threads(c->U), 0, st>>>(*c, *p, chunk);
   });
   return int(cudaGetLastError());
 }
@@ -1070,12 +1185,10 @@ int nb_kv8_append(const nb_kv8_cache* c, const nb_kv8_rows* p, cudaStream_t st) 
 int nb_kv8_truncate(const nb_kv8_cache* c, const int* len, cudaStream_t st) {
   using namespace nbk;
   if (bad_cache(c)) return -1;
-  const long stride = 0;
   const void* ptrs[2] = {c->open[0], c->open[1]};
-  const int vec = vector_of(c->D, c->type == 2 ? 4 : 2, &stride, 1, ptrs, 2);
-  const size_t smem = kBlock * (c->D | 1) * sizeof(float);
-  with_types(c->type, vec, c->code, [&](auto t, auto v, auto k) {
-    truncate_kernel<decltype(t), decltype(v)::value, decltype(k)::value><<<dim3(c->L, c->H, 2), 128, smem, st>>>(*c, len);
+  const bool pair = pairs(c->D, c->type == 2 ? 4 : 2, nullptr, 0, ptrs, 2);
+  with_types(c->type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
+    truncate_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<dim3(c->L, c->H), unit_threads(c->U), 0, st>>>(*c, len);
   });
   return int(cudaGetLastError());
 }
@@ -1084,14 +1197,12 @@ int nb_kv8_read(const nb_kv8_cache* c, const nb_kv8_rows* p, int type, cudaStrea
   using namespace nbk;
   if (bad_cache(c) || p->rows < 0) return -1;
   if (p->rows == 0) return 0;
-  const long stride = 0;
   const void* ptrs[2] = {p->dst[0], p->dst[1]};
-  const int vec = vector_of(c->D, type == 2 ? 4 : 2, &stride, 1, ptrs, 2);
-  const int chunk = p->max_rows <= 8 ? 1 : kBlock;
-  const dim3 grid((p->rows + chunk - 1) / chunk, c->H, 2);
-  const size_t smem = kBlock * (c->D | 1) * sizeof(float);
-  with_types(type, vec, c->code, [&](auto t, auto v, auto k) {
-    read_kernel<decltype(t), decltype(v)::value, decltype(k)::value><<<grid, 128, smem, st>>>(*c, *p, chunk);
+  const bool pair = pairs(c->D, type == 2 ? 4 : 2, nullptr, 0, ptrs, 2);
+  const int chunk = chunk_of(p->rows, p->max_rows, c->H);
+  const dim3 grid((p->rows + chunk - 1) / chunk, c->H);
+  with_types(type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
+    read_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<grid, unit_threads(c->U), 0, st>>>(*c, *p, chunk);
   });
   return int(cudaGetLastError());
 }
