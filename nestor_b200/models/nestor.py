@@ -279,6 +279,8 @@ class Layer(nn.Module):
         position order). Returns the gated slot updates ``[B, k, d]`` in fp32.
         """
 
+        if isinstance(cache, LayerKV8Cache):
+            return self._attention_step_kv8(n, ctx, cd, cache)
         s = self.spec
         B = n.shape[0]
         heads, hd, inner = s.heads, s.head_dim, s.heads * s.head_dim
@@ -307,6 +309,41 @@ class Layer(nn.Module):
             y = torch.einsum("bi,bdi->bd", o, wo[c]).float()
             out.append(y * ctx.gates[:, j].float().unsqueeze(-1))
         return torch.stack(out, dim=1)
+
+    def _attention_step_kv8(self, n: Tensor, ctx: "BlockContext", cd: torch.dtype, cache: "LayerKV8Cache") -> Tensor:
+        """Attention half for ``S`` new tokens of every sequence (``n [B*S, d]``) against an 8-bit cache.
+
+        The rows of the step are packed by (column, sequence) as in the full forward, appended to their lists, and each
+        attends over what its column has seen up to itself. Returns ``[B*S, k, d]`` in fp32.
+        """
+
+        s, plan = self.spec, ctx.plan
+        heads, hd, inner = s.heads, s.head_dim, s.heads * s.head_dim
+        wqkv, wo = self.qkv_weight(), self.out_weight()
+        bounds = plan.extra.get("col_bounds")
+        if bounds is None:                              # (read once for a block's layers)
+            bounds = plan.extra["col_bounds"] = plan.col_start.tolist()
+        x = n.to(cd)[plan.tok_of_row.long()]
+        qkv = x.new_empty(plan.rows, 3 * inner)
+        for c in range(s.G):
+            a, b = bounds[c], bounds[c + 1]
+            if b > a:
+                torch.matmul(x[a:b], wqkv[c].to(cd).t(), out=qkv[a:b])
+        cos, sin = ops.rope_tables(plan.pos_of_row, hd, s.rope_base)
+        qk = ops.apply_rope(qkv[:, : 2 * inner].reshape(-1, 2 * heads, hd), cos, sin)
+        v = qkv[:, 2 * inner :].view(-1, heads, hd)
+        with ops.kernel_ops(cache.kernels):
+            ops.kv8_append(cache.kv, qk[:, heads:], v, plan.seg_start, cache.count, max_rows=ctx.S)
+            cache.count = cache.count + plan.seg_start.diff()
+            o = ops.kv8_attention(qk[:, :heads], cache.kv, plan.seg_start, cache.count, 1.0 / hd, max_rows=ctx.S)
+        o = o.reshape(plan.rows, inner)
+        y = x.new_empty(plan.rows, n.shape[1])
+        for c in range(s.G):
+            a, b = bounds[c], bounds[c + 1]
+            if b > a:
+                torch.matmul(o[a:b], wo[c].to(cd).t(), out=y[a:b])
+        upd = y[plan.row_of_slot.long().reshape(-1)].view(n.shape[0], plan.k, -1).float()
+        return upd * ctx.gates.float().unsqueeze(-1)
 
     def experts(self, n: Tensor, ctx: "BlockContext", cd: torch.dtype) -> tuple[Tensor | None, Tensor, Tensor | None, dict]:
         """Expert half: ``(private [T, k, d] | None, shared [T, d], path [T, 2] | None, routing aux)``."""
@@ -368,14 +405,86 @@ class LayerKVCache:
         self.values = torch.zeros_like(self.keys)
         self.count = torch.zeros(B, G, dtype=torch.long, device=device)
 
+    def take_back(self, drop: Tensor) -> None:
+        """Forget the newest ``drop [B, G]`` entries of every list."""
+
+        self.count = self.count - drop
+
+
+class LayerKV8Cache:
+    """The same in 8 bits (``ops.KV8Cache``): one list per (column, sequence), ``list = column * B + sequence``, with
+    ``count [G * B]`` entries each. ``kernels``: whether the ops run as kernels (decided when the decode state is made, since
+    the rest of a decode step runs as PyTorch statements)."""
+
+    def __init__(self, B: int, G: int, max_len: int, heads: int, head_dim: int, device, dtype, open_dtype) -> None:
+        self.kv = ops.kv8_cache(G * B, heads, max_len, head_dim, device, dtype, open_dtype)
+        self.count = torch.zeros(G * B, dtype=torch.int32, device=self.kv.device)
+        self.kernels = ops.use_kernels(self.count)
+
+    def take_back(self, drop: Tensor) -> None:
+        self.count = self.count - drop.t().reshape(-1).to(torch.int32)
+        with ops.kernel_ops(self.kernels):
+            ops.kv8_truncate(self.kv, self.count)
+
 
 class NestorKVCache:
-    """Decode state of the whole backbone: one ``LayerKVCache`` per (block, layer)."""
+    """Decode state of the whole backbone: one ``LayerKVCache`` (``LayerKV8Cache`` for ``dtype`` int8 or float8_e4m3fn)
+    per (block, layer).
 
-    def __init__(self, backbone: "Nestor", B: int, max_len: int, device, dtype=torch.float32) -> None:
-        self.blocks = [[LayerKVCache(B, blk.spec.G, max_len, blk.spec.heads, blk.spec.head_dim, device, dtype)
-                        for _ in blk.layers] for blk in backbone.blocks]
+    ``positions [B]`` counts the tokens of every sequence and ``length`` is the largest of them. The columns of the
+    newest ``TAKE_BACK`` tokens are remembered, so that :meth:`rollback` can take tokens back (refused drafts).
+    """
+
+    TAKE_BACK = 64
+
+    def __init__(self, backbone: "Nestor", B: int, max_len: int, device, dtype=torch.float32, open_dtype=torch.float32) -> None:
+        self.eight_bit = dtype in (torch.int8, torch.float8_e4m3fn)
+
+        def layer(s):
+            if self.eight_bit:
+                return LayerKV8Cache(B, s.G, max_len, s.heads, s.head_dim, device, dtype, open_dtype)
+            return LayerKVCache(B, s.G, max_len, s.heads, s.head_dim, device, dtype)
+
+        self.blocks = [[layer(blk.spec) for _ in blk.layers] for blk in backbone.blocks]
+        self.columns = [blk.spec.G for blk in backbone.blocks]
+        self.batch, self.max_len = B, max_len
         self.length = 0
+        self.positions = torch.zeros(B, dtype=torch.long, device=device)
+        # per block, the columns [B, <= TAKE_BACK, k] of every sequence's newest tokens, oldest first (-1: none)
+        self.recent: list[Tensor | None] = [None] * len(self.blocks)
+
+    def note(self, block: int, idx: Tensor) -> None:
+        """Remember the columns ``idx [B, S, k]`` of a step's tokens in ``block``."""
+
+        old = self.recent[block]
+        self.recent[block] = (idx if old is None else torch.cat((old, idx), dim=1))[:, -self.TAKE_BACK :]
+
+    def advance(self, tokens: int) -> None:
+        self.positions = self.positions + tokens
+        self.length += tokens
+
+    def rollback(self, dropped: Tensor) -> None:
+        """Take back the newest ``dropped [B]`` tokens of every sequence (at most ``TAKE_BACK`` since they were fed)."""
+
+        dropped = dropped.to(self.positions.device, torch.long)
+        if dropped.shape != self.positions.shape:
+            raise ValueError(f"dropped must have one entry per sequence ({self.batch}), got {tuple(dropped.shape)}")
+        held = 0 if self.recent[0] is None else (self.recent[0][:, :, 0] >= 0).sum(dim=1)
+        if bool((dropped < 0).any()) or bool((dropped > held).any()):
+            raise ValueError("only tokens that the decode state remembers can be taken back (the newest "
+                             f"{self.TAKE_BACK} of a sequence, each once)")
+        for i, (rec, layers) in enumerate(zip(self.recent, self.blocks)):
+            R, k = rec.shape[1:]
+            back = torch.arange(R, device=rec.device).unsqueeze(0) - dropped.unsqueeze(1)          # where slot j moves from
+            gone = (torch.arange(R, device=rec.device).unsqueeze(0) >= R - dropped.unsqueeze(1)).unsqueeze(-1) & (rec >= 0)
+            drop = torch.zeros(self.batch, self.columns[i], dtype=torch.long, device=rec.device)
+            drop.scatter_add_(1, rec.clamp_min(0).reshape(self.batch, -1).long(), gone.reshape(self.batch, -1).long())
+            moved = rec.gather(1, back.clamp_min(0).unsqueeze(-1).expand(-1, -1, k))
+            self.recent[i] = torch.where((back >= 0).unsqueeze(-1), moved, -1)
+            for cache in layers:
+                cache.take_back(drop)
+        self.positions = self.positions - dropped
+        self.length = int(self.positions.max())
 
 
 class BlockContext:
@@ -523,7 +632,9 @@ class Block(nn.Module):
 
         s = self.spec
         idx, gates = self.route(x, noise, cd)
-        plan = ops.build_column_plan(idx.view(B, S, s.k), s.G, pos) if s.G > 1 and cache is None else None
+        # (the 8-bit decode state packs a step's rows like the full forward; a single-column block is one list per sequence)
+        packed = s.G > 1 if cache is None else isinstance(cache[0], LayerKV8Cache)
+        plan = ops.build_column_plan(idx.view(B, S, s.k), s.G, pos) if packed else None
         ctx = BlockContext(B, S, idx, gates, plan, pos)
         if not self.depth_reads:
             return self._forward_projection(x, ctx, cd, cache, idx)
@@ -857,15 +968,18 @@ class Nestor(Backbone):
     def output_dim(self) -> int:
         return self.config.output_dim
 
-    def init_kv_cache(self, batch_size: int, max_len: int, device, dtype=torch.float32) -> NestorKVCache:
-        """Empty decode state for ``batch_size`` sequences of up to ``max_len`` tokens."""
+    def init_kv_cache(self, batch_size: int, max_len: int, device, dtype=torch.float32,
+                      open_dtype=torch.float32) -> NestorKVCache:
+        """Empty decode state for ``batch_size`` sequences of up to ``max_len`` tokens. ``dtype`` int8 or float8_e4m3fn
+        keeps keys and values in 8 bits; ``open_dtype`` is then the compute dtype of the steps."""
 
-        return NestorKVCache(self, batch_size, max_len, device, dtype)
+        return NestorKVCache(self, batch_size, max_len, device, dtype, open_dtype)
 
     @torch.no_grad()
     def forward_step(self, x0: Tensor, pos: Tensor, cache: NestorKVCache, cd: torch.dtype) -> tuple[Tensor, dict]:
         """One incremental causal step: ``x0 [B, d]`` embeddings of the next token of every sequence at positions
-        ``pos [B]`` -> normalised head input ``[B, d]``, with ``cache`` updated in place.
+        ``pos [B]`` -> normalised head input ``[B, d]``, with ``cache`` updated in place. An 8-bit cache takes any number
+        ``S`` of new tokens per sequence at once (``x0 [B*S, d]``, ``pos [B, S]``).
 
         Depth reads mix a token's own sources over depth, routers and experts act per token, and a column attends
         over the members it has already seen, so feeding a sequence token by token reproduces the full forward
@@ -878,19 +992,26 @@ class Nestor(Backbone):
             raise RuntimeError("forward_step is an evaluation path: call model.eval() first")
         if not self.config.causal:
             raise RuntimeError("stepwise decoding needs a causal model: a bidirectional token sees later ones")
-        B = x0.shape[0]
+        B = cache.batch
+        S = x0.shape[0] // B
+        if x0.shape[0] != B * S or S < 1 or (S > 1 and not cache.eight_bit):
+            raise ValueError(f"a step feeds one token to each of the cache's {B} sequences"
+                             f"{', or the same number to each' if cache.eight_bit else ''}; got {x0.shape[0]} rows")
+        if cache.eight_bit and cache.length + S > cache.max_len:
+            raise ValueError(f"key/value cache of {cache.max_len} positions per column is full")
         with ops.oracle_ops():        # per-token work: the PyTorch statement of the ops on any device
             narrow, wide, x, aux = [x0], [x0], x0, []
-            for block, bcache in zip(self.blocks, cache.blocks):
-                exports, x, a = block(x, list(wide) if self.wide_reads else narrow, B, 1, cd, pos, self.column_mode, None,
+            for i, (block, bcache) in enumerate(zip(self.blocks, cache.blocks)):
+                exports, x, a = block(x, list(wide) if self.wide_reads else narrow, B, S, cd, pos, self.column_mode, None,
                                       cache=bcache)
+                cache.note(i, a["group_idx"].reshape(B, S, -1))
                 wide.extend(exports)
                 narrow = [*narrow, exports[-1]]
                 if self.block_attention_residuals is not None:
                     x = self._mix_block_outputs(len(aux), narrow)
                 aux.append(a)
             h = self._head_input(wide, narrow, x, cd)
-        cache.length += 1
+        cache.advance(S)
         return h, {"blocks": aux}
 
     def forward(self, x0: Tensor, B: int, S: int, cd: torch.dtype, pos: Tensor | None = None,

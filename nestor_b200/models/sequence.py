@@ -20,7 +20,7 @@ from nestor_b200.configs.model import (
     LanguageModelingHeadConfig, NestorConfig, ReferenceMupConfig, SequenceModelConfig, TextAdapterConfig,
 )
 from nestor_b200.models.modules import LayerStack, Matrix
-from nestor_b200.models.nestor import Nestor, W
+from nestor_b200.models.nestor import Nestor, NestorKVCache, W
 from nestor_b200.models.registry import (
     ADAPTERS, BACKBONES, HEADS, MODELS, register_adapter, register_backbone, register_head, register_model,
 )
@@ -316,37 +316,70 @@ class SequenceModel(nn.Module):
 
     # ------------------------------------------------------------------ incremental decoding
     def init_kv_cache(self, batch_size: int, max_len: int, device=None, dtype: torch.dtype = torch.float32):
+        """Empty decode state. ``dtype`` int8 or float8_e4m3fn keeps keys and values in 8 bits (``ops.kv8_attention``) and
+        lets a step feed several tokens at once."""
+
         device = self.head.weight.device if device is None else device
-        return self.backbone.init_kv_cache(batch_size, max_len, device, dtype)
+        return self.backbone.init_kv_cache(batch_size, max_len, device, dtype, open_dtype=self._step_dtype(torch.device(device)))
+
+    def _step_dtype(self, device: torch.device) -> torch.dtype:
+        return torch.float32 if self.compute_dtype is None or device.type != "cuda" else self.compute_dtype
 
     @torch.no_grad()
     def decode_step(self, ids: Tensor, cache, pos: Tensor | None = None) -> Tensor:
-        """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` (``cache`` is advanced)."""
+        """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` (``cache`` is advanced). Several tokens
+        ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n`` single steps
+        otherwise."""
 
+        if ids.dim() == 2:
+            if not cache.eight_bit:
+                steps = [self.decode_step(ids[:, t], cache, None if pos is None else pos[:, t]) for t in range(ids.shape[1])]
+                return torch.stack(steps, dim=1) if steps else ids.new_zeros(*ids.shape, self.head.vocab_size, dtype=torch.float32)
+            if ids.shape[1] == 0:
+                return ids.new_zeros(*ids.shape, self.head.vocab_size, dtype=torch.float32)
         B = ids.shape[0]
+        rows = ids.reshape(B, -1)
         if pos is None:
-            pos = torch.full((B,), cache.length, dtype=torch.long, device=ids.device)
-        cd = torch.float32 if self.compute_dtype is None else self.compute_dtype
-        if ids.device.type != "cuda":
-            cd = torch.float32
-        x0 = self.adapter(ids.reshape(B, 1)).reshape(B, -1)
+            pos = cache.positions.unsqueeze(1) + torch.arange(rows.shape[1], device=ids.device)
+            pos = pos if ids.dim() == 2 else pos.squeeze(1)
+        cd = self._step_dtype(ids.device)
+        x0 = self.adapter(rows).reshape(rows.numel(), -1)
         h, _ = self.backbone.forward_step(x0, pos, cache, cd)
-        return self.head(h, cd).float()
+        return self.head(h, cd).float().view(*ids.shape, -1)
+
+    def _prefill(self, prompt: Tensor, cache) -> Tensor | None:
+        """Feed ``prompt [B, S]`` and return the logits after its last token (``None`` for an empty prompt): pieces of up to
+        ``PREFILL`` tokens into an 8-bit cache, token by token otherwise."""
+
+        step = self.PREFILL if cache.eight_bit else 1
+        logits = None
+        for a in range(0, prompt.shape[1], step):
+            logits = self.decode_step(prompt[:, a : a + step] if step > 1 else prompt[:, a], cache)
+        return logits if logits is None or logits.dim() == 2 else logits[:, -1]
+
+    PREFILL = 512
 
     @torch.no_grad()
     def generate(self, prompt: Tensor, max_new_tokens: int, temperature: float = 0.0,
-                 generator: torch.Generator | None = None) -> Tensor:
-        """Greedy (``temperature == 0``) or sampled continuation of ``prompt [B, S0]``; returns ``[B, S0 + new]``."""
+                 generator: torch.Generator | None = None, cache_dtype: torch.dtype = torch.float32,
+                 draft: "SequenceModel | None" = None, draft_tokens: int = 4) -> Tensor:
+        """Greedy (``temperature == 0``) or sampled continuation of ``prompt [B, S0]``; returns ``[B, S0 + new]``.
 
+        ``cache_dtype`` int8 or float8_e4m3fn decodes over an 8-bit cache. With ``draft`` (a smaller model over the same
+        vocabulary) each round lets it propose ``draft_tokens`` tokens, scores them in one pass over an 8-bit cache and
+        keeps the prefix that :func:`ops.verify_draft` accepts plus one token drawn from what is left: greedy output is
+        this model's own, sampled output has its distribution, up to the arithmetic of the cache.
+        """
+
+        if draft is not None:
+            return self._generate_with_draft(prompt, max_new_tokens, temperature, generator, cache_dtype, draft, draft_tokens)
         was_training = self.training
         self.eval()
         B, S0 = prompt.shape
-        cache = self.init_kv_cache(B, S0 + max_new_tokens, prompt.device)
-        logits = None
-        for t in range(S0):
-            logits = self.decode_step(prompt[:, t], cache)
+        cache = self.init_kv_cache(B, S0 + max_new_tokens, prompt.device, cache_dtype)
+        logits = self._prefill(prompt, cache)
         out = [prompt]
-        for _ in range(max_new_tokens):
+        for i in range(max_new_tokens):
             if temperature > 0:
                 nxt = torch.multinomial(torch.softmax(logits / temperature, dim=-1), 1, generator=generator).squeeze(1)
             else:
@@ -355,6 +388,64 @@ class SequenceModel(nn.Module):
             logits = self.decode_step(nxt, cache)
         self.train(was_training)
         return torch.cat(out, dim=1)
+
+    def _generate_with_draft(self, prompt: Tensor, max_new_tokens: int, temperature: float, generator: torch.Generator | None,
+                             cache_dtype: torch.dtype, draft: "SequenceModel", n: int) -> Tensor:
+        if draft.head.vocab_size != self.head.vocab_size:
+            raise ValueError(f"the draft model has a vocabulary of {draft.head.vocab_size} tokens, this one of {self.head.vocab_size}")
+        B, S0 = prompt.shape
+        most = NestorKVCache.TAKE_BACK
+        if not 1 <= n < most:
+            raise ValueError(f"draft_tokens must be in 1..{most - 1} (a refused round has to be taken back), got {n}")
+        if S0 < 1:
+            raise ValueError("decoding with drafts needs a prompt of at least one token")
+        dev, was = prompt.device, (self.training, draft.training)
+        self.eval()
+        draft.eval()
+        room = S0 + max_new_tokens + 2 * (n + 1)      # (a sequence may overshoot by a round and then waits, feeding rounds)
+        caches = [m.init_kv_cache(B, room, dev, cache_dtype) for m in (self, draft)]
+        for m, cache in zip((self, draft), caches):
+            m._prefill(prompt[:, :-1], cache)
+        out = torch.zeros(B, room, dtype=prompt.dtype, device=dev)
+        out[:, :S0] = prompt
+        end = torch.full((B,), S0, dtype=torch.long, device=dev)             # tokens of each sequence so far
+        last = prompt[:, -1]                                                 # the newest of them: not fed yet
+        while max_new_tokens > 0 and bool((end < S0 + max_new_tokens).any()):
+            tokens, probs, cur = [], [], last
+            for i in range(n):
+                logits = draft.decode_step(cur, caches[1])
+                if temperature > 0:
+                    probs.append(torch.softmax(logits / temperature, dim=-1))
+                    cur = torch.multinomial(probs[-1], 1, generator=generator).squeeze(1)
+                else:
+                    cur = logits.argmax(dim=-1)
+                tokens.append(cur)
+            draft.decode_step(cur, caches[1])                                # (the last proposal enters its cache as well)
+            x = torch.stack(tokens, dim=1)
+            logits = self.decode_step(torch.cat((last.unsqueeze(1), x), dim=1), caches[0])
+            if temperature > 0:
+                target, q = torch.softmax(logits / temperature, dim=-1), torch.stack(probs, dim=1)
+            else:
+                target, q = torch.zeros_like(logits).scatter_(2, logits.argmax(dim=-1, keepdim=True), 1.0), None
+            u = torch.rand(B, n, generator=generator, device=dev)
+            w = torch.rand(B, generator=generator, device=dev)
+            accepted, token = ops.verify_draft(target, x, q, u, w)
+            accepted, token = accepted.long(), token.to(prompt.dtype)
+            # sequences that have their tokens wait for the others: they keep nothing of the round
+            live = end < S0 + max_new_tokens
+            new = torch.cat((x, token.unsqueeze(1)), dim=1).to(prompt.dtype)
+            new.scatter_(1, accepted.unsqueeze(1), token.unsqueeze(1))
+            at = torch.arange(n + 1, device=dev).unsqueeze(0)
+            keep = live.unsqueeze(1) & (at <= accepted.unsqueeze(1))
+            place = end.unsqueeze(1) + at
+            out.scatter_(1, place, torch.where(keep, new, out.gather(1, place)))
+            kept = torch.where(live, accepted + 1, 0)
+            end, last = end + kept, torch.where(live, token, last)
+            for cache in caches:
+                cache.rollback(n + 1 - kept)
+        self.train(was[0])
+        draft.train(was[1])
+        return out[:, : S0 + max_new_tokens]
 
     def fsdp2_wrap_order(self) -> list[nn.Module]:
         """Sharding units, in gather order: adapter, each block, backbone tail, head, root."""

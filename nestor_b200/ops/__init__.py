@@ -72,6 +72,26 @@ class oracle_ops:
         return False
 
 
+class kernel_ops:
+    """``with ops.kernel_ops(on):`` run the ops of this block as kernels (``on`` false: as PyTorch statements) whatever
+    ``oracle_ops`` region it stands in. Stepwise decoding uses it: its per-token work runs as statements, its attention over
+    an 8-bit cache as the decode state was made."""
+
+    def __init__(self, on: bool = True) -> None:
+        self.on = on
+
+    def __enter__(self):
+        global _oracle_depth
+        self.depth = _oracle_depth
+        _oracle_depth = 0 if self.on else 1
+        return self
+
+    def __exit__(self, *exc):
+        global _oracle_depth
+        _oracle_depth = self.depth
+        return False
+
+
 def use_kernels(t: torch.Tensor) -> bool:
     return t.is_cuda and not _FORCE_REF and _oracle_depth == 0
 
