@@ -116,6 +116,22 @@ def _dispatch(name: str):
     return op
 
 
+def _dispatch_first(name: str):
+    """``_dispatch`` for ops whose first argument, a tensor or a ``KV8Cache``, says where they run (a decode step calls them
+    too often to look through all of them)."""
+
+    ref_fn = getattr(_ref, name)
+
+    def op(*args, **kwargs):
+        if use_kernels(args[0] if args else next(iter(kwargs.values()))):
+            return getattr(cuda_ops(), name)(*args, **kwargs)
+        return ref_fn(*args, **kwargs)
+
+    op.__name__ = name
+    op.__doc__ = ref_fn.__doc__
+    return op
+
+
 def _eager(name: str, report_as: str):
     """An op without a fused kernel: the PyTorch statement on any device, counted in ``oracle_path_report()`` when
     it runs on CUDA tensors beside the kernels (the options that use it are outside the registered cells)."""
@@ -158,8 +174,8 @@ dense_swiglu = _dispatch("dense_swiglu")
 lm_head_ce = _dispatch("lm_head_ce")
 newton_schulz = _dispatch("newton_schulz")
 # incremental decoding: the 8-bit key/value cache, attention over it, verification of drafted tokens
-kv8_append = _dispatch("kv8_append")
-kv8_truncate = _dispatch("kv8_truncate")
-kv8_read = _dispatch("kv8_read")
-kv8_attention = _dispatch("kv8_attention")
-verify_draft = _dispatch("verify_draft")
+kv8_append = _dispatch_first("kv8_append")
+kv8_truncate = _dispatch_first("kv8_truncate")
+kv8_read = _dispatch_first("kv8_read")
+kv8_attention = _dispatch_first("kv8_attention")
+verify_draft = _dispatch_first("verify_draft")

@@ -36,6 +36,7 @@ class VerifyArgs(C.Structure):
                 ("q_row", C.c_long), ("B", C.c_int), ("n", C.c_int), ("V", C.c_int), ("type", C.c_int), ("tokens_64", C.c_int)]
 
 
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _ready = None
 
@@ -63,7 +64,7 @@ def _launch(fn, device: torch.device, *args, launches: int = 1) -> None:
 
     # (the raw-stream query costs a tenth of torch.cuda.current_stream(), which builds a Stream object)
     index = device.index
-    if torch.cuda.current_device() == index:
+    if _device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -74,7 +75,7 @@ def _launch(fn, device: torch.device, *args, launches: int = 1) -> None:
 
 
 def _cache_args(c: KV8Cache) -> CacheArgs:
-    a = c.__dict__.get("_args")          # (the fields are frozen: one argument block serves every call)
+    a = c.__dict__.get("_args")          # (the fields are fixed: one argument block serves every call)
     if a is None:
         a = CacheArgs(c.k_codes.data_ptr(), c.v_codes.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.k_open.data_ptr(),
                       c.v_open.data_ptr(), _lib.status_word(c.device).data_ptr(), c.lists, c.heads, c.blocks, c.head_dim, c.units,
@@ -123,7 +124,7 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     D.check_attention(q, cache, seg_start, lengths, scale, max_rows, out)
     given = out is not None
     if not given:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = q.new_empty(q.shape)
     if q.shape[0] == 0:
         return out
     q = _rows(q)
@@ -137,7 +138,7 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
         with torch.cuda.device(cache.device):
             size = _workspace[key] = L.nb_kv8_attention_workspace(key[0], key[1])
     # (allocated for this call on this stream: two streams, or two captured graphs, never share it)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+    ws = lengths.new_empty(size // 4)
     a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(),
                       lengths.data_ptr(), q.shape[0], max_rows, group, FLOATS[q.dtype], int(not given), scale * LOG2E)
     _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, ws.data_ptr(), size, launches=2)
@@ -148,20 +149,24 @@ def verify_draft(target_probs: Tensor, draft_tokens: Tensor, draft_probs: Tensor
                  draft_len: Tensor | None = None) -> tuple[Tensor, Tensor]:
     D.check_verify(target_probs, draft_tokens, draft_probs, accept_u, sample_u, draft_len)
     p, q = target_probs, draft_probs
-    B, n, V = p.shape[0], draft_tokens.shape[1], p.shape[2]
+    B, n, V = p.shape
+    n -= 1
     out = torch.empty(2, B, dtype=torch.int32, device=p.device)
+    accepted, token = out.unbind(0)
     if B == 0:
-        return out[0], out[1]
+        return accepted, token
     if V > 1 and p.stride(2) != 1:
         p = p.contiguous()
-    if q is not None and V > 1 and q.stride(2) != 1:
-        q = q.contiguous()
     if n == 0:
         q = None
+    elif q is not None and V > 1 and q.stride(2) != 1:
+        q = q.contiguous()
+    p_batch, p_row, _ = p.stride()
+    q_batch, q_row, _ = (0, 0, 0) if q is None else q.stride()
     draft_tokens, accept_u, sample_u = draft_tokens.contiguous(), accept_u.contiguous(), sample_u.contiguous()
+    at = out.data_ptr()
     a = VerifyArgs(p.data_ptr(), None if q is None else q.data_ptr(), draft_tokens.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(),
-                   None if draft_len is None else draft_len.data_ptr(), out.data_ptr(), out.data_ptr() + 4 * B, p.stride(0), p.stride(1),
-                   0 if q is None else q.stride(0), 0 if q is None else q.stride(1), B, n, V, FLOATS[p.dtype],
-                   int(draft_tokens.dtype == torch.int64))
+                   None if draft_len is None else draft_len.data_ptr(), at, at + 4 * B, p_batch, p_row, q_batch, q_row, B, n, V,
+                   FLOATS[p.dtype], 1 if draft_tokens.dtype == torch.int64 else 0)
     _launch(_L().nb_verify_draft, p.device, a)
-    return out[0], out[1]
+    return accepted, token

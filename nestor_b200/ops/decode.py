@@ -16,7 +16,6 @@ Kernel bodies: :mod:`nestor_b200.ops.cuda_decode`. None of these ops has a backw
 
 from __future__ import annotations
 
-import dataclasses as dc
 import math
 
 import torch
@@ -28,53 +27,49 @@ CODE_MAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 FLOATS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
-@dc.dataclass(frozen=True, eq=False)
 class KV8Cache:
     """Keys and values of ``L`` lists in 8 bits (build an empty one with :func:`kv8_cache`).
 
-    Attributes:
+    Attributes (fixed once built):
         k_codes, v_codes: ``[L, H, blocks, ceil(head_dim / 8), 512]`` int8 or float8_e4m3fn. A block's codes are units of
             8 head dims x 64 entries in the order of the kernels' matrix fragments (:func:`code_positions`).
         k_scale, v_scale: ``[L, H, blocks]`` fp32.
         k_open, v_open: ``[L, H, 2, 64, head_dim]`` originals of the youngest two blocks (block ``b`` in slot ``b % 2``),
             in the dtype of the rows that are appended (bf16, fp16 or fp32).
-        lists, heads, blocks, units, capacity, head_dim, device, dtype, open_dtype: what the tensors' shapes say.
+        lists, heads, blocks, units, capacity, head_dim, device, is_cuda, dtype, open_dtype: what the tensors say.
 
     How many entries each list holds is not part of the cache: the caller keeps ``lengths [L]`` (int32, on the device)
     and passes it, so stepping back is a smaller number plus :func:`kv8_truncate`.
     """
 
-    k_codes: Tensor
-    v_codes: Tensor
-    k_scale: Tensor
-    v_scale: Tensor
-    k_open: Tensor
-    v_open: Tensor
-
-    def __post_init__(self) -> None:
-        kc, vc, ks, vs, ko, vo = self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_open, self.v_open
-        code, kind = kc.dtype, ko.dtype
-        if code not in CODE_MAX or vc.dtype != code:
-            raise ValueError(f"cache codes are int8 or float8_e4m3fn (keys and values alike), got {code} and {vc.dtype}")
-        if kind not in FLOATS or vo.dtype != kind:
-            raise ValueError(f"the kept originals are bfloat16, float16 or float32 (keys and values alike), got {kind} and {vo.dtype}")
-        if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+    def __init__(self, k_codes: Tensor, v_codes: Tensor, k_scale: Tensor, v_scale: Tensor, k_open: Tensor, v_open: Tensor) -> None:
+        code, kind = k_codes.dtype, k_open.dtype
+        if code not in CODE_MAX or v_codes.dtype != code:
+            raise ValueError(f"cache codes are int8 or float8_e4m3fn (keys and values alike), got {code} and {v_codes.dtype}")
+        if kind not in FLOATS or v_open.dtype != kind:
+            raise ValueError(f"the kept originals are bfloat16, float16 or float32 (keys and values alike), got {kind} and {v_open.dtype}")
+        if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
             raise ValueError("cache scales are float32")
-        shape, held = kc.shape, ko.shape
+        shape, held = k_codes.shape, k_open.shape
         if len(shape) != 5 or len(held) != 5:
             raise ValueError("cache codes are [L, H, blocks, units, 512], originals [L, H, 2, 64, head_dim]")
         L, H, nb, U, _ = shape
         D = held[4]
-        if min(L, H, nb) < 1 or not 1 <= D <= MAX_HEAD_DIM or U != -(-D // 8):
+        if L < 1 or H < 1 or nb < 1 or not 1 <= D <= MAX_HEAD_DIM or U != -(-D // 8):
             raise ValueError(f"cache of {L} lists x {H} heads x {nb} blocks x {U} units for head_dim {D}: needs at least one of "
                              f"each, head_dim in 1..{MAX_HEAD_DIM} and ceil(head_dim / 8) units")
-        device = kc.device
-        for t, want in ((kc, (L, H, nb, U, 512)), (vc, shape), (ks, (L, H, nb)), (vs, (L, H, nb)), (ko, (L, H, 2, BLOCK, D)), (vo, held)):
+        device = k_codes.device
+        codes, scales, kept = (L, H, nb, U, 512), (L, H, nb), (L, H, 2, BLOCK, D)
+        for t, want in ((k_codes, codes), (v_codes, codes), (k_scale, scales), (v_scale, scales), (k_open, kept), (v_open, kept)):
             if t.shape != want or t.device != device or not t.is_contiguous():
                 raise ValueError(f"cache tensors must be contiguous, on one device and of matching shapes: got {tuple(t.shape)} on {t.device}, "
-                                 f"expected {tuple(want)} on {device}")
-        # (plain attributes: every call of every op looks them up)
-        self.__dict__.update(lists=L, heads=H, blocks=nb, units=U, capacity=nb * BLOCK, head_dim=D, device=device, dtype=code, open_dtype=kind)
+                                 f"expected {want} on {device}")
+        self.__dict__.update(k_codes=k_codes, v_codes=v_codes, k_scale=k_scale, v_scale=v_scale, k_open=k_open, v_open=v_open,
+                             lists=L, heads=H, blocks=nb, units=U, capacity=nb * BLOCK, head_dim=D, device=device,
+                             is_cuda=device.type == "cuda", dtype=code, open_dtype=kind)
+
+    def __setattr__(self, name: str, value) -> None:
+        raise AttributeError(f"the {name} of a KV8Cache is fixed (its kernels keep an argument block of it); build another one")
 
 
 def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None, dtype: torch.dtype = torch.int8,
@@ -153,18 +148,21 @@ def check_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tens
 
 def check_verify(p: Tensor, tokens: Tensor, q: Tensor | None, u: Tensor, w: Tensor, draft_len: Tensor | None) -> None:
     check_no_grad("verify_draft", p, q)
-    if p.dim() != 3 or p.shape[1] < 1 or p.shape[2] < 1 or p.dtype not in FLOATS:
-        raise ValueError(f"verify_draft: target_probs must be [B, n + 1, V] bfloat16, float16 or float32, got {tuple(p.shape)} {p.dtype}")
-    B, n, V = p.shape[0], p.shape[1] - 1, p.shape[2]
-    if tokens.shape != (B, n) or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != p.device:
-        raise ValueError(f"verify_draft: draft_tokens must be [{B}, {n}] int32 or int64 on {p.device}, got {tuple(tokens.shape)} {tokens.dtype} on {tokens.device}")
-    if q is not None and (q.shape != (B, n, V) or q.dtype != p.dtype or q.device != p.device):
-        raise ValueError(f"verify_draft: draft_probs must be [{B}, {n}, {V}] {p.dtype} on {p.device}, got {tuple(q.shape)} {q.dtype} on {q.device}")
-    for t, shape, name in ((u, (B, n), "accept_u"), (w, (B,), "sample_u")):
-        if t.shape != shape or t.dtype != torch.float32 or t.device != p.device:
-            raise ValueError(f"verify_draft: {name} must be {shape} float32 on {p.device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    shape, kind, device = p.shape, p.dtype, p.device
+    if len(shape) != 3 or shape[1] < 1 or shape[2] < 1 or kind not in FLOATS:
+        raise ValueError(f"verify_draft: target_probs must be [B, n + 1, V] bfloat16, float16 or float32, got {tuple(shape)} {kind}")
+    B, n, V = shape
+    drafted = (B, n - 1)
+    if tokens.shape != drafted or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != device:
+        raise ValueError(f"verify_draft: draft_tokens must be {drafted} int32 or int64 on {device}, got {tuple(tokens.shape)} {tokens.dtype} on {tokens.device}")
+    if q is not None and (q.shape != (B, n - 1, V) or q.dtype != kind or q.device != device):
+        raise ValueError(f"verify_draft: draft_probs must be {(B, n - 1, V)} {kind} on {device}, got {tuple(q.shape)} {q.dtype} on {q.device}")
+    if u.shape != drafted or u.dtype != torch.float32 or u.device != device:
+        raise ValueError(f"verify_draft: accept_u must be {drafted} float32 on {device}, got {tuple(u.shape)} {u.dtype} on {u.device}")
+    if w.shape != (B,) or w.dtype != torch.float32 or w.device != device:
+        raise ValueError(f"verify_draft: sample_u must be {(B,)} float32 on {device}, got {tuple(w.shape)} {w.dtype} on {w.device}")
     if draft_len is not None:
-        check_index(draft_len, B, "draft_len", p.device)
+        check_index(draft_len, B, "draft_len", device)
 
 
 # -------------------------------------------------------------------------------------- statements: the cache

@@ -188,6 +188,8 @@ def test_refusals():
         ops.kv8_cache(1, 1, 1, 129)
     with pytest.raises(ValueError, match="shapes"):
         ops.KV8Cache(cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale[:1], cache.k_open, cache.v_open)
+    with pytest.raises(AttributeError, match="fixed"):
+        cache.k_scale = cache.v_scale
     with pytest.raises(ValueError, match="scales are float32"):
         ops.KV8Cache(cache.k_codes, cache.v_codes, cache.k_scale.double(), cache.v_scale.double(), cache.k_open, cache.v_open)
     with pytest.raises(ValueError, match="k must be"):
