@@ -386,11 +386,13 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // weights down to 2^-21 of the largest keep 11 bits, and the sum of the softmax adds the rounded weights. Where the
 // output has more than bf16's 8 bits, probabilities are two fp16 numbers as well, which keeps 22.
 //
-// Division of work. All blocks of all (list, head, column tile) tasks form one line that is cut into units, whatever the
-// lengths and without the host knowing them. A warp that owns a whole task writes its output; pieces of a task that is
-// cut go to a workspace and `attn_join` adds them in order, so results do not depend on the schedule. Short lines: one
-// unit a warp. Long ones (32 blocks a warp and more): two thirds in one unit a warp, the rest in three times as many that
-// the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: 88 to 128 us).
+// Division of work, without the host knowing the lengths. Few tasks (list, head, column tile) over a short cache: a CTA
+// takes a task, its warps take equal runs of the blocks and join their results in shared memory. Otherwise all blocks of
+// all tasks form one line that is cut into units, a warp each. A warp that owns a whole task writes its output; pieces of
+// a task that is cut go to a workspace and `attn_join` adds them in order, so results do not depend on the schedule. Short
+// lines: one unit a warp. Long ones (32 blocks a warp and more): two thirds in one unit a warp, the rest in three times as
+// many that the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: 88 to 128 us). A unit
+// costs some 3 us beside its blocks (queries, scales, its piece), which shorter lines do not get back.
 constexpr float kShift = 7.f;        // log2 of the factor on the probabilities
 constexpr float kSlack = 8.f;        // how far (log2) a score may pass the running maximum; 2^(kShift + kSlack) fits fp16
 constexpr int kJoin = 4;             // warps of a CTA of attn_join
@@ -399,10 +401,11 @@ constexpr int kMaxLists = 1024;      // lists in one launch (their prefix sums s
 struct Attn {
   nb_kv8_cache c;
   nb_kv8_attn a;
-  float* ws;          // pieces: slot 2u for a task that unit u continues, 2u + 1 for one that it begins
-  long* cum;
   int* next;          // units handed out beyond the first `workers`
-  int workers, dynamic;
+  int* bad;           // whether some list's bounds were refused
+  int2* cut;          // [rows][query heads]: of the item's task the first unit; the number of pieces * 16 + the item's column
+  float* ws;          // pieces: slot 2u for a task that unit u continues, 2u + 1 for one that it begins
+  int workers, dynamic, by_task;
 };
 
 constexpr int kShares = 3;           // small units for each warp of a long line
@@ -503,6 +506,11 @@ __device__ __forceinline__ ListWork list_work(const Attn& k, int l, int end, int
   return sized(s0, s0 >= 0 && s1 <= min(k.a.rows, end) ? max(0, s1 - s0) : 0, min(max(len, 0), k.c.nb * kBlock), k.a.group, columns);
 }
 
+__device__ __forceinline__ bool covered(const Attn& k, int row, int end, int columns) {      // by a list whose bounds hold
+  const ListWork w = list_work(k, find_list(k.a.seg, k.c.L, row), end, columns);
+  return row >= w.s0 && row < w.s0 + w.n;
+}
+
 __device__ __forceinline__ float tile_max(const float (&s)[4][4], int i) {
   return fmaxf(fmaxf(fmaxf(s[0][i], s[0][2 + i]), fmaxf(s[1][i], s[1][2 + i])), fmaxf(fmaxf(s[2][i], s[2][2 + i]), fmaxf(s[3][i], s[3][2 + i])));
 }
@@ -526,20 +534,26 @@ struct Run {
   int l, h, tile, b, blocks;
   ListWork w;
 };
-__device__ __forceinline__ Run run_at(const Attn& k, const long* cum, const int* lists, long pos, long end, int columns) {
+// (By tasks the line counts tasks, and the run is the share of one of `warps` warps.)
+__device__ __forceinline__ Run run_at(const Attn& k, const long* cum, const int* lists, long pos, long end, int columns, int warp, int warps) {
   int lo = 0, hi = k.c.L;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (cum[mid] <= pos) lo = mid; else hi = mid;
   }
   const ListWork w = sized(lists[3 * lo], lists[3 * lo + 1], lists[3 * lo + 2], k.a.group, columns);
-  const int in_list = int(pos - cum[lo]), task = in_list / w.nb;
+  const int in_list = int(pos - cum[lo]), task = k.by_task ? in_list : in_list / w.nb;
   Run r;
   r.l = lo;
-  r.b = in_list - task * w.nb;
   r.h = task / w.tiles;
   r.tile = task - r.h * w.tiles;
-  r.blocks = int(min(long(w.nb - r.b), end - pos));
+  if (k.by_task) {
+    r.b = warp * w.nb / warps;
+    r.blocks = (warp + 1) * w.nb / warps - r.b;
+  } else {
+    r.b = in_list - task * w.nb;
+    r.blocks = int(min(long(w.nb - r.b), end - pos));
+  }
   r.w = w;
   return r;
 }
@@ -560,25 +574,30 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   const uint32_t half = U * 512;
   const uint32_t stage = half * HALVES;
   uint8_t* ring = smem + warp * STAGES * stage;
-  long* cum = reinterpret_cast<long*>(smem + WARPS * STAGES * stage);      // [L + 1] blocks of all tasks before list l
+  long* cum = reinterpret_cast<long*>(smem + WARPS * STAGES * stage);      // [L + 1] blocks (or tasks) before list l
   int* lists = reinterpret_cast<int*>(cum + L + 1);                         // [L][3] first row, rows, entries
   asm volatile("griddepcontrol.launch_dependents;");      // (attn_join waits for this grid before it reads what it wrote)
 
   // ---- prefix sums of the lists' work
   const int seg_end = k.a.seg[L];
+  bool bad = false;
 #pragma unroll 4
   for (int l = threadIdx.x; l < L; l += WARPS * 32) {
     const ListWork w = list_work(k, l, seg_end, COLS);
-    cum[l + 1] = w.n ? k.c.H * w.tiles * w.nb : 0;
+    cum[l + 1] = w.n ? k.c.H * w.tiles * (k.by_task ? 1 : w.nb) : 0;
     lists[3 * l] = w.s0;
     lists[3 * l + 1] = w.n;
     lists[3 * l + 2] = w.len;
-    if (blockIdx.x == 0 && (k.a.len[l] > k.c.nb * kBlock || k.a.seg[l + 1] > min(k.a.rows, seg_end) || k.a.seg[l] < 0 || k.a.seg[l + 1] < k.a.seg[l]))
-      atomicCAS(k.c.status, 0, kStatusRange);
+    bad = bad || k.a.seg[l + 1] > min(k.a.rows, seg_end) || k.a.seg[l] < 0 || k.a.seg[l + 1] < k.a.seg[l];
+    if (k.a.len[l] > k.c.nb * kBlock && blockIdx.x == 0) atomicCAS(k.c.status, 0, kStatusRange);
   }
   if (lane < STAGES) nb::mbar_init(&bars[warp][lane], 1);
   nb::fence_barrier_init();
-  __syncthreads();
+  bad = __syncthreads_or(bad);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    if (!k.by_task) *k.bad = bad;
+    if (bad) atomicCAS(k.c.status, 0, kStatusRange);
+  }
   const int each = (L + blockDim.x - 1) / blockDim.x, l0 = min(L, int(threadIdx.x) * each), l1 = min(L, l0 + each);
   long sum = 0;
   for (int l = l0; l < l1; ++l) sum += cum[l + 1];
@@ -598,20 +617,27 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   }
   if (threadIdx.x == 0) cum[0] = 0;
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int l = threadIdx.x; l <= L; l += blockDim.x) k.cum[l] = cum[l];
   const long total = cum[L];
+  if (k.by_task && (k.a.zero_tail || bad))      // (with units attn_join does this)
+    for (int r = blockIdx.x * WARPS + warp; r < k.a.rows; r += gridDim.x * WARPS)
+      if (r >= seg_end ? k.a.zero_tail : r >= k.a.seg[0] && bad && !covered(k, r, seg_end, COLS))
+        for (int i = lane; i < k.c.H * k.a.group * D; i += 32)
+          reinterpret_cast<T*>(k.a.out)[long(r) * k.a.o_row + long(i / D) * k.a.o_head + i % D] = from_f<T>(0.f);
   if (total == 0) return;
   const Cuts cuts(k, total);
   int unit = warp * gridDim.x + blockIdx.x;
-  if (unit >= cuts.workers) return;
+  if (!k.by_task && unit >= cuts.workers) return;
 
   // ---- the copies, over run and unit borders, STAGES ahead: keys of a block and its values (in one stage or in two), the
   // next block, ... A unit that the copies fetch is `unit_next` until the arithmetic gets there (units are longer than the
   // ring, so there is never more than one).
-  long feed_pos = cuts.begin(unit), feed_end = cuts.begin(unit + 1), feed_at = 0;
+  long feed_pos = 0, feed_end = 0, feed_at = 0;
   int feed_left = 0, feed_slot = 0, unit_next = -1;
-  bool feed_values = false, more = cuts.units > cuts.workers;
+  bool feed_values = false, more = !k.by_task && cuts.units > cuts.workers;
+  if (!k.by_task) {
+    feed_pos = cuts.begin(unit);
+    feed_end = cuts.begin(unit + 1);
+  }
   auto feed = [&]() {
     if (feed_left == 0) {
       if (feed_pos >= feed_end) {
@@ -625,7 +651,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
         feed_pos = cuts.begin(u);
         feed_end = cuts.begin(u + 1);
       }
-      const Run r = run_at(k, cum, lists, feed_pos, feed_end, COLS);
+      const Run r = run_at(k, cum, lists, feed_pos, feed_end, COLS, 0, 1);
       feed_at = ((long(r.l) * k.c.H + r.h) * k.c.nb + r.b) * long(half);
       feed_left = r.blocks;
       feed_pos += r.blocks;
@@ -648,8 +674,9 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     }
     feed_values = !feed_values;
   };
+  if (!k.by_task)
 #pragma unroll 1
-  for (int i = 0; i < STAGES; ++i) feed();
+    for (int i = 0; i < STAGES; ++i) feed();
   int slot = 0;
   uint32_t parity = 0;
   const uint32_t ring_at = nb::smem_u32(ring) + lane * 16;
@@ -679,7 +706,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     if (slot == 0) parity ^= 1;
   };
 
-  long pos = cuts.begin(unit), pos_end = cuts.begin(unit + 1);
+  long pos = k.by_task ? long(blockIdx.x) : cuts.begin(unit), pos_end = k.by_task ? total : cuts.begin(unit + 1);
   while (true) {
     if (pos >= pos_end) {
       if (unit_next < 0) break;
@@ -688,10 +715,17 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
       pos = cuts.begin(unit);
       pos_end = cuts.begin(unit + 1);
     }
-    const Run run = run_at(k, cum, lists, pos, pos_end, COLS);
+    const Run run = run_at(k, cum, lists, pos, pos_end, COLS, warp, WARPS);
     const ListWork w = run.w;
     const int h = run.h, tile = run.tile, b0 = run.b, b1 = run.b + run.blocks;
-    pos += run.blocks;
+    const long run_from = pos;
+    pos += k.by_task ? long(gridDim.x) : run.blocks;
+    if (k.by_task) {
+      feed_at = ((long(run.l) * k.c.H + run.h) * k.c.nb + run.b) * long(half);
+      feed_left = run.blocks;
+#pragma unroll 1
+      for (int i = 0; i < STAGES; ++i) feed();
+    }
     const long lh = long(run.l) * k.c.H + h;
     const float* ksp = k.c.scale[0] + lh * k.c.nb;
     const float* vsp = k.c.scale[1] + lh * k.c.nb;
@@ -709,14 +743,24 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     for (int nt = 0; nt < NT; ++nt) {
       const int col = tile * COLS + nt * 8 + g, a = col / k.a.group;
       const bool valid = a < w.n;
-      const long qi = valid ? long(w.s0 + a) * k.a.q_row + long(h * k.a.group + col - a * k.a.group) * k.a.q_head : 0;
+      // (columns and dims that are not there load one that is, so that all loads are in flight at once)
+      const T* from = reinterpret_cast<const T*>(k.a.q) + long(w.s0 + (valid ? a : 0)) * k.a.q_row +
+                      long(h * k.a.group + (valid ? col - a * k.a.group : 0)) * k.a.q_head;
+      T raw[PAIRS][4];
+#pragma unroll
+      for (int j = 0; j < PAIRS; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 16 * j + (i >> 1) * 8 + 2 * t + (i & 1);
+          raw[j][i] = from[d < D ? d : 0];
+        }
       float x[PAIRS][4], top = 0.f;
 #pragma unroll
       for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = 16 * j + (i >> 1) * 8 + 2 * t + (i & 1);
-          x[j][i] = valid && d < D ? to_f(reinterpret_cast<const T*>(k.a.q)[qi + d]) : 0.f;
+          x[j][i] = valid && d < D ? to_f(raw[j][i]) : 0.f;
           top = fmaxf(top, fabsf(x[j][i]));
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -960,18 +1004,22 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     }
 
     // ---- the piece's result
-    const bool whole = b0 == 0 && b1 == w.nb;
-    float* to_piece = k.ws + long(2 * unit + (b0 == 0 ? 1 : 0)) * COLS * (8 * U + 2);
+    const bool whole = !k.by_task && b0 == 0 && b1 == w.nb;
+    const int width = 8 * U + 2;
+    // (by tasks into the warp's own ring, which holds nothing by now)
+    float* to_piece = k.by_task ? reinterpret_cast<float*>(ring) : k.ws + long(2 * unit + (b0 == 0 ? 1 : 0)) * COLS * width;
+    int pieces = 1;
+    if (!whole && !k.by_task && b0 == 0) pieces = cuts.of(run_from + w.nb - 1) - unit + 1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float z = sm[nt][i];
-        const int in_tile = nt * 8 + 2 * t + i, c = tile * COLS + in_tile, row = c / k.a.group;
+        const int in_tile = nt * 8 + 2 * t + i, c = tile * COLS + in_tile, row = c / k.a.group, head = h * k.a.group + c - row * k.a.group;
         if (row >= w.n) continue;
         if (whole) {
           const float inv = z == 0.f ? 0.f : kUnit / z;
-          const long at = long(w.s0 + row) * k.a.o_row + long(h * k.a.group + c - row * k.a.group) * k.a.o_head;
+          const long at = long(w.s0 + row) * k.a.o_row + long(head) * k.a.o_head;
 #pragma unroll
           for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
@@ -980,7 +1028,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
               if (d < D) reinterpret_cast<T*>(k.a.out)[at + d] = from_f<T>(o[j][nt][2 * q + i] * inv);
             }
         } else {
-          float* to = to_piece + in_tile * (8 * U + 2);
+          float* to = to_piece + in_tile * width;
 #pragma unroll
           for (int j = 0; j < PAIRS; ++j)
 #pragma unroll
@@ -991,77 +1039,92 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
             to[8 * U + 1] = z;
           }
         }
+        if (!k.by_task && b0 == 0 && g == 0) k.cut[long(w.s0 + row) * k.c.H * k.a.group + head] = make_int2(unit, pieces * 16 + in_tile);
       }
+    if (k.by_task) {
+      __syncthreads();
+      const int n = min(COLS, w.n * k.a.group - tile * COLS);
+      for (int i = threadIdx.x; i < n * D; i += WARPS * 32) {
+        const int in_tile = i / D, d = i - in_tile * D, c = tile * COLS + in_tile, row = c / k.a.group;
+        const float* from = reinterpret_cast<const float*>(smem) + in_tile * width;
+        float top = -INFINITY, x = 0.f, z = 0.f;
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) top = fmaxf(top, from[q * (STAGES * stage / 4) + 8 * U]);
+#pragma unroll
+        for (int q = 0; q < WARPS; ++q) {
+          const float m = from[q * (STAGES * stage / 4) + 8 * U], f = m == top ? 1.f : ex2(m - top);
+          x += f * from[q * (STAGES * stage / 4) + d];
+          z += f * from[q * (STAGES * stage / 4) + 8 * U + 1];
+        }
+        reinterpret_cast<T*>(k.a.out)[long(w.s0 + row) * k.a.o_row + long(h * k.a.group + c - row * k.a.group) * k.a.o_head + d] =
+            from_f<T>(z == 0.f ? 0.f : x / z);
+      }
+      nb::fence_async_smem();      // (the rings are written by copies again)
+      __syncthreads();
+    }
   }
 }
 
 // Adds the pieces of each (row, query head) whose task was cut, in their order. TEAM warps share an item: 4 where there
 // are few items (their tasks are cut into many pieces then), else 1. Rows behind the last list become zeros when
-// `zero_tail` is set. Launched so that it starts under the main kernel's end: up to the wait it reads the caller's
-// tensors only.
+// `zero_tail` is set. What it is bound by is the chain of loads behind the main kernel's end: the item's cut, then all
+// pieces at once.
 template <int TEAM>
 __global__ void __launch_bounds__(kJoin * 32) attn_join(const Attn k, int cols) {
-  __shared__ float red[kJoin], sums[kJoin], acc_s[kJoin][128];
+  __shared__ float tops[kJoin], sums[kJoin], acc_s[kJoin][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM, heads = k.c.H * k.a.group;
   const long item = blockIdx.x * long(kJoin / TEAM) + warp / TEAM;
   const int row = int(item / heads), head = int(item - long(row) * heads);
-  const int L = k.c.L, D = k.c.D, width = 8 * k.c.U + 2;
-  const int seg_begin = k.a.seg[0], seg_end = k.a.seg[L];
-  bool live = item < long(k.a.rows) * heads && row >= seg_begin && row < seg_end;
-  const bool tail = k.a.zero_tail && item < long(k.a.rows) * heads && row >= seg_end;
+  const int L = k.c.L, D = k.c.D, width = 8 * k.c.U + 2, seg_begin = k.a.seg[0], seg_end = k.a.seg[L];
+  const bool exists = item < long(k.a.rows) * heads;
+  bool live = exists && row >= seg_begin && row < seg_end;
   const long at = long(row) * k.a.o_row + long(head) * k.a.o_head;
-  const int l = find_list(k.a.seg, L, live ? row : seg_begin);
-  const ListWork w = list_work(k, l, seg_end, cols);
-  const bool refused = live && (row < w.s0 || row >= w.s0 + w.n);      // bounds that the main kernel refused
-  if (tail || refused)
-    for (int d = lane + 32 * member; d < D; d += 32 * TEAM) store_any(k.a.out, at + d, k.a.q_type, 0.f);
-  live = live && !refused;
-  const int h = head / k.a.group, col = (row - w.s0) * k.a.group + head - h * k.a.group;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int u0 = 0, n = 0;
-  if (live) {
-    const Cuts cuts(k, k.cum[L]);
-    const long begin = k.cum[l] + (long(h) * w.tiles + col / cols) * w.nb;
-    u0 = cuts.of(begin);
-    n = cuts.of(begin + w.nb - 1) - u0 + 1;
+  const int2 cut = live ? k.cut[item] : make_int2(0, 0);
+  bool zero = exists && k.a.zero_tail && row >= seg_end;
+  if (*k.bad && live && !covered(k, row, seg_end, cols)) {
+    live = false;
+    zero = true;
   }
-  if (TEAM == 1 ? n <= 1 : __syncthreads_and(n <= 1)) return;
-  auto piece = [&](int i) { return k.ws + (long(2 * (u0 + i) + (i == 0 ? 1 : 0)) * cols + col % cols) * width; };
-  float top = -INFINITY;
-  for (int i = lane + 32 * member; i < n; i += 32 * TEAM) top = fmaxf(top, piece(i)[8 * k.c.U]);
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-  if constexpr (TEAM > 1) {
-    if (lane == 0) red[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < TEAM; ++i) top = fmaxf(top, red[i]);
-  }
-  float acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  if (zero)
+    for (int d = lane + 32 * member; d < D; d += 32 * TEAM) store_any(k.a.out, at + d, k.a.q_type, 0.f);
+  const int n = live ? cut.y >> 4 : 0, col = cut.y & 15;      // (at most 16 columns a tile)
+  if (n <= 1) return;                  // (with TEAM > 1 the CTA has one item)
+  float top = -INFINITY, acc[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
 #pragma unroll 4
   for (int i = member; i < n; i += TEAM) {
-    const float* from = piece(i);
-    const float m = from[8 * k.c.U], f = m == top ? 1.f : ex2(m - top);
-    sum += f * from[8 * k.c.U + 1];
+    const float* from = k.ws + (long(2 * (cut.x + i) + (i == 0 ? 1 : 0)) * cols + col) * width;
+    const float m = from[8 * k.c.U], z = from[8 * k.c.U + 1];
+    float x[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (lane + 32 * q < D) acc[q] += f * from[lane + 32 * q];
+    for (int q = 0; q < 4; ++q) x[q] = lane + 32 * q < D ? from[lane + 32 * q] : 0.f;
+    const float now = fmaxf(top, m), keep = top == now ? 1.f : ex2(top - now), f = m == now ? 1.f : ex2(m - now);
+    top = now;
+    sum = sum * keep + f * z;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc[q] = acc[q] * keep + f * x[q];
   }
   if constexpr (TEAM > 1) {
 #pragma unroll
     for (int q = 0; q < 4; ++q) acc_s[warp][lane + 32 * q] = acc[q];
-    if (lane == 0) sums[warp] = sum;
-    __syncthreads();
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < TEAM; ++i) sum += sums[i];
-    const int d = threadIdx.x;       // (128 threads, at most 128 dims)
-    if (d < D) {
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < TEAM; ++i) x += acc_s[i][d];
-      store_any(k.a.out, at + d, k.a.q_type, sum == 0.f ? 0.f : x / sum);
+    if (lane == 0) {
+      tops[warp] = top;
+      sums[warp] = sum;
     }
+    __syncthreads();
+    top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) top = fmaxf(top, tops[i]);
+    float x = 0.f;
+    sum = 0.f;
+    const int d = threadIdx.x;         // (128 threads, at most 128 dims)
+#pragma unroll
+    for (int i = 0; i < TEAM; ++i) {
+      const float f = tops[i] == top ? 1.f : ex2(tops[i] - top);
+      sum += f * sums[i];
+      x += f * acc_s[i][d];
+    }
+    if (d < D) store_any(k.a.out, at + d, k.a.q_type, sum == 0.f ? 0.f : x / sum);
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -1083,7 +1146,7 @@ AttnFn pick_code(int code, int type) {
 
 // Column tiles of 8: one for single tokens, two when several rows or shared heads bring more columns (a converted
 // block then serves both); four would not fit the registers of the wider heads.
-int tiles_for(int columns) { return columns <= 8 ? 1 : 2; }
+int tiles_for(long columns) { return columns <= 8 ? 1 : 2; }
 
 int width_of(int U) { return U <= 5 ? 5 : U <= 8 ? 8 : U <= 10 ? 10 : 16; }
 
@@ -1120,7 +1183,6 @@ cudaError_t allow_smem(AttnFn fn, int which) {
 }
 
 long slot_floats(int U, int cols) { return long(cols) * (8 * U + 2); }
-long workers_of(int U, int nt) { return long(multiprocessors()) * warps_of(width_of(U), nt); }
 
 
 // Whether every pair of dims (2i, 2i + 1) of every row is aligned to the pair's size.
@@ -1207,54 +1269,85 @@ int nb_kv8_read(const nb_kv8_cache* c, const nb_kv8_rows* p, int type, cudaStrea
   return int(cudaGetLastError());
 }
 
-// Bytes of workspace that an attention call over heads of D dims takes for `columns` query columns a list and head.
-long nb_kv8_attention_workspace(int D, int columns) {
-  using namespace nbk;
-  const int U = (D + 7) / 8, nt = tiles_for(columns);
-  return 16 + (kMaxLists + 2) * 8 + workers_of(U, nt) * (1 + kShares) * 2 * slot_floats(U, 8 * nt) * 4;
+}      // extern "C"
+namespace nbk {
+// What the host knows of an attention call: tile columns, whether a CTA takes whole tasks, the most tasks, the workspace.
+struct Plan {
+  int nt, cols, width, warps, sms;
+  bool by_task;
+  long tasks, bytes;
+};
+Plan plan_of(int L, int H, int nb, int D, int rows, int max_rows, int group) {
+  Plan p;
+  const int U = (D + 7) / 8;
+  const long columns = std::min(long(max_rows), long(rows)) * group;
+  p.nt = tiles_for(columns);
+  p.cols = 8 * p.nt;
+  p.width = width_of(U);
+  p.warps = warps_of(p.width, p.nt);
+  p.sms = multiprocessors();
+  p.tasks = std::min(long(rows) * group, std::min(long(rows), long(L)) * ((columns + p.cols - 1) / p.cols)) * H;
+  // by tasks: at most two a CTA and four blocks a warp (4096 entries of a narrow head). 80 lists x 3 heads of 2000 entries:
+  // BYTASK us against BYUNIT by units; beyond that the longest task would decide.
+  p.by_task = L <= kMaxLists && nb <= 4 * p.warps && p.tasks <= 2l * p.sms;
+  p.bytes = p.by_task ? 0 : 16 + 8l * rows * H * group + long(p.sms) * p.warps * (1 + kShares) * 2 * slot_floats(U, p.cols) * 4;
+  return p;
+}
+}      // namespace nbk
+extern "C" {
+
+// Bytes of workspace that such an attention call takes (0: none).
+long nb_kv8_attention_workspace(int L, int H, int nb, int D, int rows, int max_rows, int group) {
+  return nbk::plan_of(L, H, nb, D, rows, max_rows, group).bytes;
 }
 
 int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long ws_bytes, cudaStream_t st) {
   using namespace nbk;
-  if (bad_cache(c) || a->rows < 0 || a->group < 1) return -1;
+  if (bad_cache(c) || a->rows < 0 || a->group < 1 || a->max_rows < 1) return -1;
   // (a list's tasks are counted in 32 bits)
   if (long(c->H) * ((long(a->rows) * a->group + 7) / 8) * c->nb > 0x7fffffffl) return -3;
   if (a->rows == 0) return 0;
-  const long columns = long(a->max_rows) * a->group;
-  const int nt = tiles_for(columns > 1024 ? 1024 : int(columns)), cols = 8 * nt, width = width_of(c->U);
-  AttnFn fn = pick(c->U, nt, c->code, a->q_type);
-  const int warps = warps_of(width, nt), L_smem = c->L < kMaxLists ? c->L : kMaxLists;
-  const size_t smem = size_t(warps) * stages_of(width) * halves_of(width) * c->U * 512 + 8 + L_smem * 20;
-  cudaError_t rc = allow_smem(fn, variant(c->U, nt, c->code, a->q_type));
+  const Plan plan = plan_of(c->L, c->H, c->nb, c->D, a->rows, a->max_rows, a->group);
+  if (plan.bytes > ws_bytes) return -2;
+  AttnFn fn = pick(c->U, plan.nt, c->code, a->q_type);
+  const int L_smem = c->L < kMaxLists ? c->L : kMaxLists;
+  const size_t smem = size_t(plan.warps) * stages_of(plan.width) * halves_of(plan.width) * c->U * 512 + 8 + L_smem * 20;
+  cudaError_t rc = allow_smem(fn, variant(c->U, plan.nt, c->code, a->q_type));
   if (rc != cudaSuccess) return int(rc);
-  const int sms = multiprocessors(), all = sms * warps;
   Attn k;
+  k.c = *c;
+  k.a = *a;
+  k.by_task = plan.by_task;
+  k.dynamic = k.workers = 0;
+  k.next = k.bad = nullptr;
+  k.cut = nullptr;
+  k.ws = nullptr;
+  if (plan.by_task) {
+    fn<<<int(std::min(long(plan.sms), plan.tasks)), plan.warps * 32, smem, st>>>(k);
+    return int(cudaGetLastError());
+  }
   k.next = reinterpret_cast<int*>(ws);
-  k.cum = reinterpret_cast<long*>(reinterpret_cast<char*>(ws) + 16);
-  k.ws = reinterpret_cast<float*>(k.cum + kMaxLists + 2);
-  if (nb_kv8_attention_workspace(c->D, nt * 8) > ws_bytes) return -2;
+  k.bad = k.next + 1;
+  k.cut = reinterpret_cast<int2*>(k.next + 4);
+  const long items = long(a->rows) * c->H * a->group;
+  k.ws = reinterpret_cast<float*>(k.cut + items);
   for (int l0 = 0; l0 < c->L; l0 += kMaxLists) {      // (more lists than one launch holds: slices, in stream order)
-    k.c = *c;
-    k.a = *a;
     k.c.L = c->L - l0 < kMaxLists ? c->L - l0 : kMaxLists;
     const long lh = long(l0) * c->H * c->nb;
     for (int i = 0; i < 2; ++i) {
       k.c.codes[i] = reinterpret_cast<uint8_t*>(c->codes[i]) + lh * c->U * 512;
       k.c.scale[i] = c->scale[i] + lh;
     }
-    k.a.seg += l0;
-    k.a.len += l0;
+    k.a.seg = a->seg + l0;
+    k.a.len = a->len + l0;
     k.a.zero_tail = a->zero_tail && l0 + k.c.L >= c->L;
-    // the most blocks that this slice can have, as far as the host knows
-    const long most_tasks = std::min(long(a->rows) * a->group, std::min(long(a->rows), long(k.c.L)) * ((columns + cols - 1) / cols)) * c->H;
-    k.dynamic = most_tasks * c->nb >= long(kLong) * all;
+    k.dynamic = plan.tasks * c->nb >= long(kLong) * plan.sms * plan.warps;
     if (k.dynamic && (rc = cudaMemsetAsync(k.next, 0, sizeof(int), st)) != cudaSuccess) return int(rc);
-    const int grid = k.dynamic ? sms : int(std::min(long(sms), std::max(most_tasks * c->nb, 1l)));
-    k.workers = grid * warps;
-    fn<<<grid, warps * 32, smem, st>>>(k);
+    const int grid = k.dynamic ? plan.sms : int(std::min(long(plan.sms), std::max(plan.tasks * c->nb, 1l)));
+    k.workers = grid * plan.warps;
+    fn<<<grid, plan.warps * 32, smem, st>>>(k);
     if ((rc = cudaGetLastError()) != cudaSuccess) return int(rc);
-    const long items = long(a->rows) * c->H * a->group;
-    const bool teams = items <= 16l * sms;
+    const bool teams = items <= 16l * plan.sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(teams ? items : (items + kJoin - 1) / kJoin));
     cfg.blockDim = dim3(kJoin * 32);
@@ -1264,7 +1357,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    rc = teams ? cudaLaunchKernelEx(&cfg, attn_join<kJoin>, (const Attn)k, cols) : cudaLaunchKernelEx(&cfg, attn_join<1>, (const Attn)k, cols);
+    rc = teams ? cudaLaunchKernelEx(&cfg, attn_join<kJoin>, (const Attn)k, plan.cols) : cudaLaunchKernelEx(&cfg, attn_join<1>, (const Attn)k, plan.cols);
     if (rc != cudaSuccess) return int(rc);
   }
   return 0;

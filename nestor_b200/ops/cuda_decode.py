@@ -50,7 +50,7 @@ def _L():
         L.nb_kv8_truncate.argtypes = [p(CacheArgs), vp, vp]
         L.nb_kv8_read.argtypes = [p(CacheArgs), p(RowArgs), C.c_int, vp]
         L.nb_kv8_attention.argtypes = [p(CacheArgs), p(AttentionArgs), vp, C.c_long, vp]
-        L.nb_kv8_attention_workspace.argtypes = [C.c_int, C.c_int]
+        L.nb_kv8_attention_workspace.argtypes = [C.c_int] * 7
         L.nb_verify_draft.argtypes = [p(VerifyArgs), vp]
         for f in (L.nb_kv8_append, L.nb_kv8_truncate, L.nb_kv8_read, L.nb_kv8_attention, L.nb_verify_draft):
             f.restype = C.c_int
@@ -116,7 +116,6 @@ def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype
 
 
 LOG2E = math.log2(math.e)
-_workspace: dict[tuple[int, int, int], int] = {}
 
 
 def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor, scale: float, max_rows: int = 1,
@@ -125,23 +124,26 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     given = out is not None
     if not given:
         out = q.new_empty(q.shape)
-    if q.shape[0] == 0:
+    rows = q.shape[0]
+    if rows == 0:
         return out
     q = _rows(q)
     q_row, q_head, _ = q.stride()
     o_row, o_head, _ = out.stride()
-    L = _L()
     group = q.shape[1] // cache.heads
-    key = (cache.head_dim, min(max_rows * group, 32), cache.device.index)
-    size = _workspace.get(key)
-    if size is None:
-        with torch.cuda.device(cache.device):
-            size = _workspace[key] = L.nb_kv8_attention_workspace(key[0], key[1])
+    L = _L()
+    index = cache.device.index
+    if _device() == index:
+        size = L.nb_kv8_attention_workspace(cache.lists, cache.heads, cache.blocks, cache.head_dim, rows, max_rows, group)
+    else:
+        with torch.cuda.device(index):
+            size = L.nb_kv8_attention_workspace(cache.lists, cache.heads, cache.blocks, cache.head_dim, rows, max_rows, group)
     # (allocated for this call on this stream: two streams, or two captured graphs, never share it)
-    ws = lengths.new_empty(size // 4)
-    a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(),
-                      lengths.data_ptr(), q.shape[0], max_rows, group, FLOATS[q.dtype], int(not given), scale * LOG2E)
-    _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, ws.data_ptr(), size, launches=2)
+    ws = lengths.new_empty(-(-size // 4)) if size else None
+    a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(), lengths.data_ptr(), rows,
+                      max_rows, group, FLOATS[q.dtype], 0 if given else 1, scale * LOG2E)
+    _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, None if ws is None else ws.data_ptr(), size,
+            launches=1 if ws is None else 2)
     return out
 
 
