@@ -87,6 +87,17 @@ __device__ __forceinline__ float2 floats(float2 v, float) { return v; }
 __device__ __forceinline__ void make_zero(unsigned& v) { v = 0u; }
 __device__ __forceinline__ void make_zero(float2& v) { v = make_float2(0.f, 0.f); }
 
+// larger of a and |v|, element by element (a NaN stays)
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned v, __nv_bfloat16) {
+  const __nv_bfloat162 m = __hmax2_nan(reinterpret_cast<const __nv_bfloat162&>(a), __habs2(reinterpret_cast<const __nv_bfloat162&>(v)));
+  return reinterpret_cast<const unsigned&>(m);
+}
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned v, __half) {
+  const __half2 m = __hmax2_nan(reinterpret_cast<const __half2&>(a), __habs2(reinterpret_cast<const __half2&>(v)));
+  return reinterpret_cast<const unsigned&>(m);
+}
+__device__ __forceinline__ float2 larger(float2 a, float2 v, float) { return make_float2(max_nan(a.x, fabsf(v.x)), max_nan(a.y, fabsf(v.y))); }
+
 template <typename T, bool PAIR>
 __device__ __forceinline__ Two<T> load_two(const T* p, bool second) {
   if constexpr (PAIR) return *reinterpret_cast<const Two<T>*>(p);
@@ -138,17 +149,24 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
   // (entries and dims that are not there load one that is, so that all loads are in flight at once, and become zeros)
   Two<T> x[2][NU][8];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv)
+  for (int kv = 0; kv < 2; ++kv) {
+    const T* held = reinterpret_cast<const T*>(src[kv].held) + g * D;
+    const T* rows = reinterpret_cast<const T*>(src[kv].rows) + (g - t0) * src[kv].row_stride;
+    const T* first = t0 ? reinterpret_cast<const T*>(src[kv].held) : reinterpret_cast<const T*>(src[kv].rows);
+    const long step = 8 * src[kv].row_stride;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int e = min(8 * i + g, n - 1);
-      const T* from = e < t0 ? reinterpret_cast<const T*>(src[kv].held) + e * D : reinterpret_cast<const T*>(src[kv].rows) + (e - t0) * src[kv].row_stride;
+      const int e = 8 * i + g;
+      const T* from = e >= n ? first : e < t0 ? held : rows;
+      held += 8 * D;
+      rows += step;
 #pragma unroll
       for (int a = 0; a < NU; ++a) {
         const int d = 8 * (warp + a * warps) + 2 * t;
         x[kv][a][i] = load_two<T, PAIR>(from + (d < D ? d : 0), d + 1 < D);
       }
     }
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
@@ -158,14 +176,14 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
         for (int kv = 0; kv < 2; ++kv) make_zero(x[kv][a][i]);
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
-    float top = 0.f;
+    Two<T> tops;
+    make_zero(tops);
 #pragma unroll
     for (int a = 0; a < NU; ++a)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 y = floats(x[kv][a][i], T{});
-        top = max_nan(top, max_nan(fabsf(y.x), fabsf(y.y)));
-      }
+      for (int i = 0; i < 8; ++i) tops = larger(tops, x[kv][a][i], T{});
+    const float2 both = floats(tops, T{});
+    float top = max_nan(both.x, both.y);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, s));
     if (lane == 0) red[kv][warp] = top;
@@ -193,8 +211,12 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
     const bool poison = !(amax < INFINITY), empty = amax < 0x1p-100f;
     const float fit = poison || empty ? 0.f : __fdiv_rn(Q, amax);
     uint4* out = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(c.codes[kv]) + (lh * c.nb + b) * (long(c.U) * 512)) + lane;
-    if (threadIdx.x == 0)
-      c.scale[kv][lh * c.nb + b] = poison ? __uint_as_float(0x7fc00000u) : (empty ? 0.f : __fdiv_rn(amax, Q));
+    if (threadIdx.x == 0) c.scale[kv][lh * c.nb + b] = poison ? __uint_as_float(0x7fc00000u) : (empty ? 0.f : __fdiv_rn(amax, Q));
+    if (poison)      // (zero times a NaN is a NaN: the codes are made zero)
+#pragma unroll
+      for (int a = 0; a < NU; ++a)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) make_zero(x[kv][a][i]);
 #pragma unroll
     for (int a = 0; a < NU; ++a) {
       const int u = warp + a * warps;
@@ -205,8 +227,7 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float2 v = floats(x[kv][a][2 * w + i], T{});
-          // (zero times a poisoned block's NaN is a NaN: its codes are made zero)
-          half[i] = code_pair<CODE>(poison ? make_float2(0.f, 0.f) : make_float2(__fmul_rn(v.x, fit), __fmul_rn(v.y, fit)));
+          half[i] = code_pair<CODE>(make_float2(__fmul_rn(v.x, fit), __fmul_rn(v.y, fit)));
           if (kv == 1) half[i] = transpose8x8(__byte_perm(half[i], 0u, 0x4140));
         }
         word[w] = __byte_perm(half[0], half[1], kv == 0 ? 0x5410 : 0x6420);
@@ -216,7 +237,8 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
   }
 }
 
-// grid (ceil(rows / chunk), H), a warp for each unit or two. A CTA looks through its chunk of rows for those that begin a
+// grid ceil(rows / chunk) * H (the heads of a row are neighbours, in memory and in time), a warp for each unit or two. A
+// CTA looks through its chunk of rows for those that begin a
 // block or a list and stores the block that each of them begins; the others exit. The two youngest blocks' new rows are
 // kept as originals, by the CTA that stores the block. One case is different: an append that begins inside a block b0
 // and goes on to b0 + 2 and further. Those blocks take the slot from which b0's older originals are read, so the CTA of
@@ -224,9 +246,9 @@ __device__ __forceinline__ void store_block(const nb_kv8_cache& c, long lh, int 
 template <typename T, bool PAIR, int CODE, int NU>
 __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) append_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
   __shared__ float red[2][2][8];
-  const int h = blockIdx.y, cap = c.nb * kBlock, D = c.D;
+  const int h = blockIdx.x % c.H, cap = c.nb * kBlock, D = c.D;
   const int end = min(p.seg[c.L], p.rows);
-  int r = blockIdx.x * chunk, turn = 0;
+  int r = int(blockIdx.x / c.H) * chunk, turn = 0;
   const int r1 = min(r + chunk, end);
   const T* rows[2] = {reinterpret_cast<const T*>(p.src[0]) + h * p.head_stride[0], reinterpret_cast<const T*>(p.src[1]) + h * p.head_stride[1]};
   while (r < r1) {
@@ -308,7 +330,7 @@ __device__ __forceinline__ float2 decoded(unsigned pair) {         // of codes i
 template <typename T, bool PAIR, int CODE, int NU>
 __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p, int chunk) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, g = lane >> 2, t = lane & 3;
-  const int h = blockIdx.y, cap = c.nb * kBlock, D = c.D;
+  const int h = blockIdx.x % c.H, cap = c.nb * kBlock, D = c.D;
   const int end = max(0, min(p.seg[c.L], p.rows));
   T* dst[2] = {reinterpret_cast<T*>(p.dst[0]) + long(h) * D, reinterpret_cast<T*>(p.dst[1]) + long(h) * D};
   const long rs = long(c.H) * D;
@@ -319,7 +341,7 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
       dst[0][at] = dst[1][at] = from_f<T>(0.f);
     }
   };
-  int r = blockIdx.x * chunk;
+  int r = int(blockIdx.x / c.H) * chunk;
   const int r_end = min(r + chunk, p.rows), r1 = min(r_end, end);
   if (r_end > max(r, end)) zeros(max(r, end), r_end);
   while (r < r1) {
@@ -1237,9 +1259,10 @@ int nb_kv8_append(const nb_kv8_cache* c, const nb_kv8_rows* p, cudaStream_t st) 
   const void* ptrs[4] = {p->src[0], p->src[1], c->open[0], c->open[1]};
   const bool pair = pairs(c->D, c->type == 2 ? 4 : 2, strides, 4, ptrs, 4);
   const int chunk = chunk_of(p->rows, p->max_rows, c->H);
-  const dim3 grid((p->rows + chunk - 1) / chunk, c->H);
+  const long grid = (long(p->rows) + chunk - 1) / chunk * c->H;
+  if (grid > 0x7fffffffl) return -1;
   with_types(c->type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
-    append_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<grid, unit_threads(c->U), 0, st>>>(*c, *p, chunk);
+    append_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<unsigned(grid), unit_threads(c->U), 0, st>>>(*c, *p, chunk);
   });
   return int(cudaGetLastError());
 }
@@ -1262,9 +1285,10 @@ int nb_kv8_read(const nb_kv8_cache* c, const nb_kv8_rows* p, int type, cudaStrea
   const void* ptrs[2] = {p->dst[0], p->dst[1]};
   const bool pair = pairs(c->D, type == 2 ? 4 : 2, nullptr, 0, ptrs, 2);
   const int chunk = chunk_of(p->rows, p->max_rows, c->H);
-  const dim3 grid((p->rows + chunk - 1) / chunk, c->H);
+  const long grid = (long(p->rows) + chunk - 1) / chunk * c->H;
+  if (grid > 0x7fffffffl) return -1;
   with_types(type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
-    read_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<grid, unit_threads(c->U), 0, st>>>(*c, *p, chunk);
+    read_kernel<decltype(t), decltype(v)::value, decltype(k)::value, decltype(n)::value><<<unsigned(grid), unit_threads(c->U), 0, st>>>(*c, *p, chunk);
   });
   return int(cudaGetLastError());
 }
