@@ -23,7 +23,7 @@
 namespace nbv {
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kMaxCluster = 8;
+constexpr int kMaxCluster = 8;
 constexpr int kMaxSpans = 1024;      // spans of a row: their sums (8 KB) stand in every CTA's shared memory
 
 __device__ __forceinline__ float val(const float* p, long i) { return __ldg(p + i); }
@@ -31,34 +31,53 @@ __device__ __forceinline__ float val(const __half* p, long i) { return __half2fl
 __device__ __forceinline__ float val(const __nv_bfloat16* p, long i) { return __bfloat162float(p[i]); }
 
 // What vocabulary entry j weighs in the draw. MODE 0: p. 1: max(p - q, 0). 2: p without entry `skip`.
-template <typename T, int MODE>
-__device__ __forceinline__ float weight(const T* p, const T* q, long skip, int j) {
-  const float x = val(p, j);
-  if constexpr (MODE == 1) {
-    const float y = val(q, j);
-    return x > y ? __fsub_rn(x, y) : 0.f;
+// Weights of the N rows of 32 entries from j0 on, entry j0 + 32 i + lane in w[i]; nothing behind b. Every load is made
+// (behind b of the last entry), so that all of them are in flight at once.
+template <typename T, int MODE, int N>
+__device__ __forceinline__ void load_weights(float (&w)[N], const T* p, const T* q, long skip, int j0, int b) {
+  const int lane = threadIdx.x & 31;
+  float x[N], y[N];
+  const bool whole = j0 + 32 * N <= b;
+  if (whole) {
+    p += j0 + lane;
+    if constexpr (MODE == 1) q += j0 + lane;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      x[i] = val(p, 32 * i);
+      if constexpr (MODE == 1) y[i] = val(q, 32 * i);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int j = min(j0 + 32 * i + lane, b - 1);
+      x[i] = val(p, j);
+      if constexpr (MODE == 1) y[i] = val(q, j);
+    }
   }
-  if constexpr (MODE == 2) return x > 0.f && j != skip ? x : 0.f;
-  return x > 0.f ? x : 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (MODE == 1) w[i] = x[i] > y[i] ? __fsub_rn(x[i], y[i]) : 0.f;
+    else w[i] = x[i] > 0.f && !(MODE == 2 && j0 + 32 * i + lane == skip) ? x[i] : 0.f;
+  }
+  if (!whole)
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (j0 + 32 * i + lane >= b) w[i] = 0.f;
 }
 
-// Sum of entries [a, b), lane by lane with stride 32.
+// Sum of entries [a, b), a < b, lane by lane with stride 32.
 template <typename T, int MODE>
 __device__ __forceinline__ double span_sum(const T* p, const T* q, long skip, int a, int b) {
-  const int lane = threadIdx.x & 31;
   double s0 = 0., s1 = 0.;
-  int j = a + lane;
-  for (; j + 7 * 32 < b; j += 8 * 32) {
-    float w[8];
+  for (int j = a; j < b; j += 512) {
+    float w[16];
+    load_weights<T, MODE>(w, p, q, skip, j, b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = weight<T, MODE>(p, q, skip, j + 32 * i);
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
+    for (int i = 0; i < 16; i += 2) {
       s0 += double(w[i]);
       s1 += double(w[i + 1]);
     }
   }
-  for (; j < b; j += 32) s0 += double(weight<T, MODE>(p, q, skip, j));
   s0 += s1;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) s0 += __shfl_xor_sync(0xffffffffu, s0, d);
@@ -74,12 +93,9 @@ __device__ __forceinline__ int find_entry(const T* p, const T* q, long skip, int
   for (int j0 = a; j0 < b; j0 += 256) {
     float w[8];
     double s[8];
+    load_weights<T, MODE>(w, p, q, skip, j0, b);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int j = j0 + 32 * i + lane;
-      w[i] = j < b ? weight<T, MODE>(p, q, skip, j) : 0.f;
-      s[i] = w[i];
-    }
+    for (int i = 0; i < 8; ++i) s[i] = w[i];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1)
 #pragma unroll
@@ -101,8 +117,9 @@ __device__ __forceinline__ int find_entry(const T* p, const T* q, long skip, int
 
 // Draws from the row; returns false if nothing weighs anything. All CTAs of the cluster call it together. Span i belongs
 // to warp i % (warps of the cluster); a CTA keeps the sums of its spans at their places in `all` and copies the others'.
-template <typename T, int MODE>
+template <typename T, int MODE, int THREADS>
 __device__ __forceinline__ bool draw(const nb_verify_args& a, int span, const T* p, const T* q, long skip, float w, int b, double* all) {
+  constexpr int kThreads = THREADS, kWarps = THREADS / 32;
   cg::cluster_group cluster = cg::this_cluster();
   const int CL = cluster.num_blocks(), rank = cluster.block_rank();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, V = a.V;
@@ -158,8 +175,8 @@ __device__ __forceinline__ bool draw(const nb_verify_args& a, int span, const T*
   return true;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const nb_verify_args a, int span) {
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const nb_verify_args a, int span) {
   __shared__ double all[kMaxSpans];
   cg::cluster_group cluster = cg::this_cluster();
   const int b = blockIdx.x / cluster.num_blocks(), lane = threadIdx.x & 31;
@@ -169,18 +186,16 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const nb_verify_arg
   auto token = [&](int i) {
     return a.tokens_64 ? reinterpret_cast<const long long*>(a.tokens)[long(b) * a.n + i] : (long long)(reinterpret_cast<const int*>(a.tokens)[long(b) * a.n + i]);
   };
-  // ---- the accepted prefix (every warp for itself)
+  // ---- the accepted prefix (every warp for itself; tokens behind `len` are loaded beside it and not looked at)
   int accepted = len;
-  for (int i0 = 0; i0 < len; i0 += 32) {
-    const int i = i0 + lane;
-    bool ok = true;
-    if (i < len) {
-      const long long x = token(i);
-      const bool known = x >= 0 && x < a.V;
-      const float px = known ? val(P + i * a.p_row, x) : 0.f;
-      const float qx = !Q ? 1.f : (known ? val(Q + i * a.q_row, x) : 0.f);
-      ok = __fmul_rn(a.u[long(b) * a.n + i], qx) < px;
-    }
+  for (int i0 = 0; i0 < a.n && i0 < len; i0 += 32) {
+    const int i = i0 + lane, at = min(i, a.n - 1);
+    const long long x = token(at);
+    const float u = a.u[long(b) * a.n + at];
+    const bool known = x >= 0 && x < a.V;
+    const float px = known ? val(P + at * a.p_row, x) : 0.f;
+    const float qx = !Q ? 1.f : (known ? val(Q + at * a.q_row, x) : 0.f);
+    const bool ok = i >= len || __fmul_rn(u, qx) < px;
     const unsigned refused = ~__ballot_sync(0xffffffffu, ok);
     if (refused) {
       accepted = i0 + __ffs(refused) - 1;
@@ -191,10 +206,10 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const nb_verify_arg
   const T* p = P + accepted * a.p_row;
   const float w = a.w[b];
   bool done;
-  if (accepted == len) done = draw<T, 0>(a, span, p, nullptr, -1, w, b, all);
+  if (accepted == len) done = draw<T, 0, THREADS>(a, span, p, nullptr, -1, w, b, all);
   else {
-    done = Q ? draw<T, 1>(a, span, p, Q + accepted * a.q_row, -1, w, b, all) : draw<T, 2>(a, span, p, nullptr, token(accepted), w, b, all);
-    if (!done) done = draw<T, 0>(a, span, p, nullptr, -1, w, b, all);
+    done = Q ? draw<T, 1, THREADS>(a, span, p, Q + accepted * a.q_row, -1, w, b, all) : draw<T, 2, THREADS>(a, span, p, nullptr, token(accepted), w, b, all);
+    if (!done) done = draw<T, 0, THREADS>(a, span, p, nullptr, -1, w, b, all);
   }
   if (cluster.block_rank() == 0 && threadIdx.x == 0) {
     a.accepted[b] = accepted;
@@ -208,18 +223,20 @@ extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
   using namespace nbv;
   if (a->B < 0 || a->n < 0 || a->V < 1 || a->V > (1 << 30) || a->type < 0 || a->type > 2) return -1;
   if (a->B == 0) return 0;
-  // spans that keep the sums within their 8 KB, and no more CTAs a row than there are spans for half of their warps or than
-  // fit the GPU at once (4 an SM): a second wave would wait for its first loads while the first one's end idles
+  // Spans that keep the sums within their 8 KB, and no more CTAs a row than there are spans for half of their warps or than
+  // fit the GPU at once: a second wave would wait for its first loads while the first one's end idles (256 rows of
+  // 100263: 45 us in one wave, 48 to 63 in more). Many rows take CTAs of 4 warps instead of 8, which spread evenly.
   int span = 512;
   while ((a->V + span - 1) / span > kMaxSpans) span *= 2;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const int threads = long(a->B) * kMaxCluster > 4l * sms ? 128 : 256, warps = threads / 32;
   int cl = 1;
-  while (cl < kMaxCluster && cl * kWarps * span < 2 * a->V && long(a->B) * cl * 2 <= 4l * sms) cl *= 2;
+  while (cl < kMaxCluster && long(cl) * warps * span < 2l * a->V && long(a->B) * cl * 2 <= long(1024 / threads) * sms) cl *= 2;
   if (long(a->B) * cl > 0x7fffffffl) return -1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a->B) * cl);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -227,9 +244,10 @@ extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t rc = a->type == 0   ? cudaLaunchKernelEx(&cfg, verify_kernel<__nv_bfloat16>, *a, span)
-                   : a->type == 1 ? cudaLaunchKernelEx(&cfg, verify_kernel<__half>, *a, span)
-                                  : cudaLaunchKernelEx(&cfg, verify_kernel<float>, *a, span);
+  using Fn = void (*)(const nb_verify_args, int);
+  const Fn fn = threads == 256 ? (a->type == 0 ? verify_kernel<__nv_bfloat16, 256> : a->type == 1 ? verify_kernel<__half, 256> : verify_kernel<float, 256>)
+                               : (a->type == 0 ? verify_kernel<__nv_bfloat16, 128> : a->type == 1 ? verify_kernel<__half, 128> : verify_kernel<float, 128>);
+  const cudaError_t rc = cudaLaunchKernelEx(&cfg, fn, *a, span);
   if (rc != cudaSuccess) return int(rc);
   return int(cudaGetLastError());
 }

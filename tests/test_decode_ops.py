@@ -638,6 +638,17 @@ def test_verification_kernel(kind, V):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_verification_kernel_on_many_sequences(kind):
+    for B, n, V, greedy in ((300, 2, 5003, False), (90, 3, 50257, False), (700, 1, 130, True)):
+        p, x, q, u, w, lens = drafts(B, n, V, kind, greedy, B)
+        want = ops.verify_draft(p, x, q, u, w, lens)
+        d = lambda t: None if t is None else t.to(DEV)              # noqa: E731
+        got = ops.verify_draft(d(p), d(x), d(q), d(u), d(w), d(lens))
+        assert torch.equal(want[0], got[0].cpu()) and torch.equal(want[1], got[1].cpu())
+
+
+@pytest.mark.gpu
 def test_borders_of_verification_kernel():
     for p, x, q, u, w, accepted, token in edge_cases():
         d = lambda t: None if t is None else t.to(DEV)              # noqa: E731
