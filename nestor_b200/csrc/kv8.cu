@@ -412,9 +412,10 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // takes a task, its warps take equal runs of the blocks and join their results in shared memory. Otherwise all blocks of
 // all tasks form one line that is cut into units, a warp each. A warp that owns a whole task writes its output; pieces of
 // a task that is cut go to a workspace and `attn_join` adds them in order, so results do not depend on the schedule. Short
-// lines: one unit a warp. Long ones (32 blocks a warp and more): two thirds in one unit a warp, the rest in three times as
-// many that the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: 88 to 128 us). A unit
-// costs some 3 us beside its blocks (queries, scales, its piece), which shorter lines do not get back.
+// lines: one unit a warp. Long ones (32 blocks a warp and more): five sixths in one unit a warp, the rest in as many
+// smaller ones that the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: the last warp
+// at 128 us instead of 117). A unit costs some 3 us beside its blocks (queries, scales, its piece) and twice the units cost
+// the join 4 us: a line of 20 blocks a warp took 92 us so and takes 80 without, and more and smaller units lost as well.
 constexpr float kShift = 7.f;        // log2 of the factor on the probabilities
 constexpr float kSlack = 8.f;        // how far (log2) a score may pass the running maximum; 2^(kShift + kSlack) fits fp16
 constexpr int kJoin = 4;             // warps of a CTA of attn_join
@@ -430,8 +431,8 @@ struct Attn {
   int workers, dynamic, by_task;
 };
 
-constexpr int kShares = 3;           // small units for each warp of a long line
-constexpr int kLong = 32;            // blocks a warp from which on a line is long (a small unit has 3 blocks then)
+constexpr int kShares = 1;           // small units for each warp of a long line
+constexpr int kLong = 32;            // blocks a warp from which on a line is long (a small unit has 5 blocks then)
 struct Cuts {
   long total, head;                  // blocks; those in the first `workers` units
   int workers, units;
@@ -439,7 +440,7 @@ struct Cuts {
     if (k.dynamic && t >= long(kLong) * k.workers) {
       workers = k.workers;
       units = (1 + kShares) * workers;
-      head = t - t / 3;
+      head = t - t / 6;
     } else {
       units = workers = int(max(1l, min(long(k.workers), t)));
       head = t;
@@ -1119,7 +1120,7 @@ __global__ void __launch_bounds__(kJoin * 32) attn_join(const Attn k, int cols) 
     const float m = from[8 * k.c.U], z = from[8 * k.c.U + 1];
     float x[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) x[q] = lane + 32 * q < D ? from[lane + 32 * q] : 0.f;
+    for (int q = 0; q < 4; ++q) x[q] = from[min(lane + 32 * q, D - 1)];      // (no branch: the loads of four pieces are in flight at once)
     const float now = fmaxf(top, m), keep = top == now ? 1.f : ex2(top - now), f = m == now ? 1.f : ex2(m - now);
     top = now;
     sum = sum * keep + f * z;
@@ -1311,8 +1312,9 @@ Plan plan_of(int L, int H, int nb, int D, int rows, int max_rows, int group) {
   p.warps = warps_of(p.width, p.nt);
   p.sms = multiprocessors();
   p.tasks = std::min(long(rows) * group, std::min(long(rows), long(L)) * ((columns + p.cols - 1) / p.cols)) * H;
-  // by tasks: at most two a CTA and four blocks a warp (4096 entries of a narrow head). 80 lists x 3 heads of 2000 entries:
-  // BYTASK us against BYUNIT by units; beyond that the longest task would decide.
+  // by tasks: at most two a CTA and four blocks a warp (4096 entries of a narrow head); beyond that the longest task would
+  // decide. 80 lists x 3 heads of 2000 entries take 16.7 us instead of 18.5, 8 x 2 of 400 7.1 instead of 8.8, and a call
+  // costs the host 19 us instead of 23 (one launch, no workspace).
   p.by_task = L <= kMaxLists && nb <= 4 * p.warps && p.tasks <= 2l * p.sms;
   p.bytes = p.by_task ? 0 : 16 + 8l * rows * H * group + long(p.sms) * p.warps * (1 + kShares) * 2 * slot_floats(U, p.cols) * 4;
   return p;
@@ -1371,7 +1373,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
     k.workers = grid * plan.warps;
     fn<<<grid, plan.warps * 32, smem, st>>>(k);
     if ((rc = cudaGetLastError()) != cudaSuccess) return int(rc);
-    const bool teams = items <= 16l * plan.sms;
+    const bool teams = items <= 32l * plan.sms;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(teams ? items : (items + kJoin - 1) / kJoin));
     cfg.blockDim = dim3(kJoin * 32);

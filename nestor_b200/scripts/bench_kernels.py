@@ -3,7 +3,7 @@
 ``python -m nestor_b200.scripts.bench_kernels [case ...] [--reps N]`` prints one line per kernel launch
 shape: time, achieved TFLOP/s or GB/s and the fraction of the measured peaks in ``MEASURED_PEAKS.json``
 (fallback 1590 TFLOP/s, 6650 GB/s). Cases: ``gemm`` (expert / attention / head GEMMs of nestor_200m),
-``flash``, ``depth``, ``ns`` (Newton-Schulz), ``gather`` (all-gather fused into the bank GEMMs, one GPU), ``small`` /
+``flash``, ``depth``, ``ns`` (Newton-Schulz), ``decode`` (8-bit cache: append, read, attention; draft verification), ``gather`` (all-gather fused into the bank GEMMs, one GPU), ``small`` /
 ``gather-small`` (one launch of each, sized for a profiler capture). Inputs are larger
 than the 126 MB L2 or an L2 flush is written between repetitions.
 """
@@ -194,6 +194,47 @@ def case_gather(reps: int, small: bool = False) -> None:
         report(f"down, weights staged (ring {ring})", timed(lambda: down(spec), reps), 2.0 * rows * d * h)
 
 
+@torch.no_grad()
+def case_decode(reps: int) -> None:
+    """One layer of a decode step of 64 sequences over 12288 entries a list (the first block's 3 of 8 columns), a prompt of
+    8 x 4096 tokens entering its lists, and the verification of 4 drafted tokens of 256 sequences."""
+
+    from nestor_b200 import ops
+    _, bw, src = peaks()
+
+    def report(name, ms, nbytes):
+        print(f"  {name:58s} {ms * 1e3:8.1f} us  {nbytes / ms / 1e6:7.0f} GB/s ({nbytes / ms / 1e6 / bw:.2f} of {src})", flush=True)
+
+    H, hd, n = 5, 40, 12288
+    for code in (torch.int8, torch.float8_e4m3fn):
+        cache = ops.kv8_cache(192, H, n + 64, hd, "cuda", code)
+        seg, start = torch.arange(193, dtype=torch.int32, device="cuda"), torch.full((192,), n, dtype=torch.int32, device="cuda")
+        q, k, v = (torch.randn(192, H, hd, device="cuda").to(BF) for _ in range(3))
+        fill = torch.randn(192 * 4096, H, hd, device="cuda").to(BF)
+        for a in range(0, n, 4096):
+            ops.kv8_append(cache, fill, fill, torch.arange(0, 192 * 4096 + 1, 4096, dtype=torch.int32, device="cuda"),
+                           torch.full((192,), a, dtype=torch.int32, device="cuda"), max_rows=4096)
+        report(f"append, 192 rows, {code}", timed(lambda: ops.kv8_append(cache, k, v, seg, start), reps), 192 * H * hd * 2 * 3)
+        report(f"attention, 192 rows x {n}, {code}", timed(lambda: ops.kv8_attention(q, cache, seg, start + 1, 1 / hd), reps),
+               192 * H * n * (2 * hd + 8 / 64))
+        del cache, fill
+    rows = 8 * 6 * 4096
+    cache = ops.kv8_cache(64, 3, 4096, hd, "cuda")
+    seg = torch.arange(0, rows + 1, rows // 64, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(64, dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(rows, 3, hd, device="cuda").to(BF) for _ in range(2))
+    report(f"append, {rows} rows", timed(lambda: ops.kv8_append(cache, k, v, seg, zero, max_rows=4096), reps), rows * 3 * hd * 2 * 3)
+    report(f"read, {rows} rows", timed(lambda: ops.kv8_read(cache, seg, zero, rows, dtype=BF), reps), rows * 3 * hd * 2 * 3)
+    B, V = 256, 100263
+    p = torch.softmax(torch.randn(B, 5, V, device="cuda") * 2.5, dim=-1)
+    d = torch.softmax(torch.log(p[:, :4]) + torch.randn(B, 4, V, device="cuda") * 0.5, dim=-1)
+    x = torch.multinomial(d.view(-1, V), 1).view(B, 4)
+    u, w = torch.rand(B, 4, device="cuda"), torch.rand(B, device="cuda")
+    accepted, _ = ops.verify_draft(p, x, d, u, w)
+    nbytes = float((2 - (accepted == 4).float()).sum()) * V * 4
+    report(f"verification, {B} x 4 drafts, vocabulary {V}", timed(lambda: ops.verify_draft(p, x, d, u, w), reps), nbytes)
+
+
 def main(argv: list[str] | None = None) -> None:
     ap = argparse.ArgumentParser(description=__doc__.split("\n")[0])
     ap.add_argument("cases", nargs="*", default=["gemm", "flash", "depth"])
@@ -207,7 +248,7 @@ def main(argv: list[str] | None = None) -> None:
         if c == "small":
             case_gemm(a.reps, small=True); case_flash(a.reps, small=True); case_depth(a.reps, small=True); case_ns(a.reps, small=True)
         else:
-            {"gemm": case_gemm, "flash": case_flash, "depth": case_depth, "gather": case_gather, "ns": case_ns,
+            {"gemm": case_gemm, "flash": case_flash, "depth": case_depth, "gather": case_gather, "ns": case_ns, "decode": case_decode,
              "gather-small": lambda r: case_gather(r, small=True)}[c](a.reps)
     from nestor_b200.ops import _lib
     _lib.check_status(torch.device("cuda"))
