@@ -1245,7 +1245,7 @@ int chunk_of(int rows, int max_rows, int heads) {
 }
 
 bool bad_cache(const nb_kv8_cache* c) {
-  return c->D < 1 || c->D > 128 || c->U != (c->D + 7) / 8 || c->H < 1 || c->H > 65535 || c->L < 1 || c->nb < 1 || !c->status || c->code < 0 || c->code > 1;
+  return c->D < 1 || c->D > 128 || c->U != (c->D + 7) / 8 || c->H < 1 || c->H > 65535 || c->L < 1 || c->nb < 1 || c->nb >= (1 << 25) || !c->status || c->code < 0 || c->code > 1;
 }
 
 }  // namespace nbk

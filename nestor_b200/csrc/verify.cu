@@ -56,8 +56,10 @@ __device__ __forceinline__ void load_weights(float (&w)[N], const T* p, const T*
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    if constexpr (MODE == 1) w[i] = x[i] > y[i] ? __fsub_rn(x[i], y[i]) : 0.f;
-    else w[i] = x[i] > 0.f && !(MODE == 2 && j0 + 32 * i + lane == skip) ? x[i] : 0.f;
+    if constexpr (MODE == 1) {
+      y[i] = fmaxf(y[i], 0.f);      // (a NaN counts as zero)
+      w[i] = x[i] > y[i] ? __fsub_rn(x[i], y[i]) : 0.f;
+    } else w[i] = x[i] > 0.f && !(MODE == 2 && j0 + 32 * i + lane == skip) ? x[i] : 0.f;
   }
   if (!whole)
 #pragma unroll
@@ -193,8 +195,8 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) verify_kernel(const n
     const long long x = token(at);
     const float u = a.u[long(b) * a.n + at];
     const bool known = x >= 0 && x < a.V;
-    const float px = known ? val(P + at * a.p_row, x) : 0.f;
-    const float qx = !Q ? 1.f : (known ? val(Q + at * a.q_row, x) : 0.f);
+    const float px = known ? fmaxf(val(P + at * a.p_row, x), 0.f) : 0.f;      // (a NaN counts as zero)
+    const float qx = !Q ? 1.f : (known ? fmaxf(val(Q + at * a.q_row, x), 0.f) : 0.f);
     const bool ok = i >= len || __fmul_rn(u, qx) < px;
     const unsigned refused = ~__ballot_sync(0xffffffffu, ok);
     if (refused) {

@@ -331,6 +331,8 @@ class SequenceModel(nn.Module):
         ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n`` single steps
         otherwise."""
 
+        if ids.shape[0] != cache.batch:
+            raise ValueError(f"the cache decodes {cache.batch} sequences, got tokens for {ids.shape[0]}")
         if ids.dim() == 2:
             if not cache.eight_bit:
                 steps = [self.decode_step(ids[:, t], cache, None if pos is None else pos[:, t]) for t in range(ids.shape[1])]

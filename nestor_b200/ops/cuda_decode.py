@@ -95,7 +95,7 @@ def kv8_append(cache: KV8Cache, k: Tensor, v: Tensor, seg_start: Tensor, start: 
     k, v = _rows(k), _rows(v)
     (k_row, k_head, _), (v_row, v_head, _) = k.stride(), v.stride()
     a = RowArgs(k.data_ptr(), v.data_ptr(), k_row, v_row, k_head, v_head, None, None, seg_start.data_ptr(), start.data_ptr(),
-                k.shape[0], max_rows)
+                k.shape[0], min(max_rows, k.shape[0]))
     _launch(_L().nb_kv8_append, cache.device, _cache_args(cache), a)
 
 
@@ -106,11 +106,11 @@ def kv8_truncate(cache: KV8Cache, lengths: Tensor) -> None:
 
 def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype: torch.dtype = torch.float32,
              max_rows: int = BLOCK) -> tuple[Tensor, Tensor]:
-    D.check_read(cache, seg_start, start, rows, dtype)
+    D.check_read(cache, seg_start, start, rows, dtype, max_rows)
     k = torch.empty(rows, cache.heads, cache.head_dim, dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
     if rows:
-        a = RowArgs(None, None, 0, 0, 0, 0, k.data_ptr(), v.data_ptr(), seg_start.data_ptr(), start.data_ptr(), rows, max_rows)
+        a = RowArgs(None, None, 0, 0, 0, 0, k.data_ptr(), v.data_ptr(), seg_start.data_ptr(), start.data_ptr(), rows, min(max_rows, 1 << 30))
         _launch(_L().nb_kv8_read, cache.device, _cache_args(cache), a, FLOATS[dtype])
     return k, v
 
@@ -130,7 +130,7 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     q = _rows(q)
     q_row, q_head, _ = q.stride()
     o_row, o_head, _ = out.stride()
-    group = q.shape[1] // cache.heads
+    group, max_rows = q.shape[1] // cache.heads, min(max_rows, rows)
     L = _L()
     index = cache.device.index
     if _device() == index:

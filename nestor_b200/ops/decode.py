@@ -64,6 +64,10 @@ class KV8Cache:
             if t.shape != want or t.device != device or not t.is_contiguous():
                 raise ValueError(f"cache tensors must be contiguous, on one device and of matching shapes: got {tuple(t.shape)} on {t.device}, "
                                  f"expected {want} on {device}")
+        if k_codes.data_ptr() % 16 or v_codes.data_ptr() % 16:
+            raise ValueError("cache codes must begin on a 16-byte boundary")
+        if nb * BLOCK >= 2 ** 31:
+            raise ValueError(f"a list holds fewer than 2^31 entries, got {nb} blocks")
         self.__dict__.update(k_codes=k_codes, v_codes=v_codes, k_scale=k_scale, v_scale=v_scale, k_open=k_open, v_open=v_open,
                              lists=L, heads=H, blocks=nb, units=U, capacity=nb * BLOCK, head_dim=D, device=device,
                              is_cuda=device.type == "cuda", dtype=code, open_dtype=kind)
@@ -84,7 +88,11 @@ def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None,
     codes = lambda: torch.zeros(lists, heads, nb, -(-head_dim // 8), 512, dtype=torch.uint8, device=device).view(dtype)   # noqa: E731
     scale = lambda: torch.zeros(lists, heads, nb, dtype=torch.float32, device=device)                       # noqa: E731
     held = lambda: torch.zeros(lists, heads, 2, BLOCK, head_dim, dtype=open_dtype, device=device)           # noqa: E731
-    return KV8Cache(codes(), codes(), scale(), scale(), held(), held())
+    cache = KV8Cache(codes(), codes(), scale(), scale(), held(), held())
+    if cache.is_cuda:
+        from nestor_b200.ops import _lib
+        _lib.status_word(cache.device)           # (made here, not by a first step that may be under graph capture)
+    return cache
 
 
 # ----------------------------------------------------------------------------- argument checks (both bodies)
@@ -98,6 +106,13 @@ def check_no_grad(op: str, *tensors: Tensor | None) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{op} is a decoding op without a backward pass: call it under torch.no_grad()")
+
+
+def check_count(op: str, rows: int, max_rows: int) -> None:
+    if max_rows < 1:
+        raise ValueError(f"{op}: max_rows must be at least 1, got {max_rows}")
+    if not 0 <= rows < 2 ** 31:
+        raise ValueError(f"{op}: rows must be in 0..2^31 - 1, got {rows}")
 
 
 def check_rows(op: str, t: Tensor, name: str, cache: KV8Cache) -> None:
@@ -115,15 +130,13 @@ def check_append(cache: KV8Cache, k: Tensor, v: Tensor, seg_start: Tensor, start
         raise ValueError(f"kv8_append: {k.shape[0]} rows of keys but {v.shape[0]} of values")
     check_index(seg_start, cache.lists + 1, "seg_start", cache.device)
     check_index(start, cache.lists, "start", cache.device)
-    if max_rows < 1:
-        raise ValueError(f"max_rows must be at least 1, got {max_rows}")
+    check_count("kv8_append", k.shape[0], max_rows)
 
 
-def check_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype: torch.dtype) -> None:
+def check_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype: torch.dtype, max_rows: int) -> None:
     check_index(seg_start, cache.lists + 1, "seg_start", cache.device)
     check_index(start, cache.lists, "start", cache.device)
-    if rows < 0:
-        raise ValueError(f"rows must not be negative, got {rows}")
+    check_count("kv8_read", rows, max_rows)
     if dtype not in FLOATS:
         raise ValueError(f"kv8_read writes bfloat16, float16 or float32, got {dtype}")
 
@@ -139,11 +152,15 @@ def check_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tens
     check_index(lengths, cache.lists, "lengths", cache.device)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"kv8_attention: scale must be positive and finite, got {scale}")
-    if max_rows < 1:
-        raise ValueError(f"max_rows must be at least 1, got {max_rows}")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (out.shape[2] > 1 and out.stride(2) != 1)):
-        raise ValueError(f"kv8_attention: out must have the shape, dtype and device of q and contiguous heads, got {tuple(out.shape)} "
-                         f"{out.dtype} on {out.device}")
+    check_count("kv8_attention", shape[0], max_rows)
+    if cache.heads * -(-shape[0] * (shape[1] // cache.heads) // 8) * cache.blocks >= 2 ** 31:
+        raise ValueError(f"kv8_attention: {shape[0]} rows x {shape[1]} heads over {cache.blocks} blocks are too many for one call: pass them in parts")
+    if out is not None:
+        step = out.stride()
+        if (out.shape != shape or out.dtype != q.dtype or out.device != q.device or (shape[2] > 1 and step[2] != 1)
+                or (shape[0] > 1 and step[0] == 0) or (shape[1] > 1 and step[1] == 0)):
+            raise ValueError(f"kv8_attention: out must have the shape, dtype and device of q, contiguous heads and rows of its own, got "
+                             f"{tuple(out.shape)} {out.dtype} on {out.device}, strides {step}")
 
 
 def check_verify(p: Tensor, tokens: Tensor, q: Tensor | None, u: Tensor, w: Tensor, draft_len: Tensor | None) -> None:
@@ -283,7 +300,7 @@ def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype
     """The values that stand in the cache: keys and values ``[rows, H, head_dim]`` of entries ``start[l] .. start[l] + n``
     of every list, packed by ``seg_start``; rows behind ``seg_start[-1]`` are zeros. ``max_rows`` only steers speed."""
 
-    check_read(cache, seg_start, start, rows, dtype)
+    check_read(cache, seg_start, start, rows, dtype, max_rows)
     seg, at = _bounds(cache, seg_start, start, rows)
     out = []
     for which in ("k", "v"):
@@ -363,7 +380,7 @@ def verify_draft(target_probs: Tensor, draft_tokens: Tensor, draft_probs: Tensor
         if draft_probs is None:
             rest = torch.where(torch.arange(V, device=dev) == x[b, i].unsqueeze(1), 0.0, r)
         else:
-            rest = (r - flush(draft_probs[b, i].float())).clamp_min(0.0)
+            rest = flush(r - flush(draft_probs[b, i].float()))
         use = (a < length) & (rest > 0).any(dim=1)
         r = torch.where(use.unsqueeze(1), rest, r)
     run = r.double().cumsum(dim=1)

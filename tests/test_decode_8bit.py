@@ -81,6 +81,8 @@ def test_steps_of_several_tokens_match_the_full_forward(family, tiny_scale, monk
     assert cache.length == 24 and cache.positions.tolist() == [24, 24]
     with pytest.raises(ValueError, match="cache"):
         m.decode_step(ids[:, :1], cache)
+    with pytest.raises(ValueError, match="tokens for 4"):
+        m.decode_step(torch.cat((ids, ids))[:, 0], m.init_kv_cache(2, 8, dtype=torch.int8))
 
 
 @pytest.mark.parametrize("eight_bit", [True, False])

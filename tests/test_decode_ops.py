@@ -214,15 +214,19 @@ def test_refusals():
         ops.kv8_truncate(cache, i32([0, 129]))
     with pytest.raises(ValueError, match="kv8_read writes"):
         ops.kv8_read(cache, seg, start, 2, dtype=torch.int8)
-    with pytest.raises(ValueError, match="rows must not"):
+    with pytest.raises(ValueError, match="rows must be in"):
         ops.kv8_read(cache, seg, start, -1)
     for q in (row[:, :2], row[..., :8], row.double()):
         with pytest.raises(ValueError, match="q must be"):
             ops.kv8_attention(q, cache, seg, start, 1.0)
     with pytest.raises(ValueError, match="scale"):
         ops.kv8_attention(row, cache, seg, start, 0.0)
-    with pytest.raises(ValueError, match="out must"):
-        ops.kv8_attention(row, cache, seg, start, 1.0, out=row.float())
+    for out in (row.float(), row[:1].expand(2, 3, 16), torch.zeros(2, 3, 32, dtype=torch.bfloat16)[..., ::2]):
+        with pytest.raises(ValueError, match="out must"):
+            ops.kv8_attention(row, cache, seg, start, 1.0, out=out)
+    with pytest.raises(ValueError, match="16-byte"):
+        odd = torch.zeros(cache.k_codes.numel() + 1, dtype=torch.int8)[1:].view(cache.k_codes.shape)
+        ops.KV8Cache(odd, cache.v_codes, cache.k_scale, cache.v_scale, cache.k_open, cache.v_open)
     with pytest.raises(ValueError, match="exceeds the key/value cache"):
         ops.kv8_attention(row, cache, seg, i32([0, 129]), 1.0)
     with pytest.raises(RuntimeError, match="no_grad"):
@@ -318,6 +322,10 @@ def edge_cases():
         (*one(9, [1.0, 0.0, 0.0, 0.0], 0.0, 0.0), 0, 1),
         (*one(0, None, 0.1, 1.0), 1, 3),                             # out of range: the last entry with mass
         (p * 0, torch.tensor([[1]]), None, torch.tensor([[0.0]]), torch.tensor([0.5]), 0, -1),        # no mass at all
+        (torch.tensor([[[0.5, math.nan, 0.5, 0.0], [0.0, 0.25, 0.0, 0.75]]]), torch.tensor([[1]]), torch.tensor([[[0.6, 0.2, math.nan, 0.0]]]),
+         torch.tensor([[0.1]]), torch.tensor([0.9]), 0, 2),          # a NaN in p is refused, one in q takes nothing off
+        (torch.tensor([[[0.5, 0.0, 0.5, 0.0], [0.0, 0.25, 0.0, 0.75]]]), torch.tensor([[2]]), torch.tensor([[[0.6, 0.2, math.nan, 0.0]]]),
+         torch.tensor([[0.1]]), torch.tensor([0.2]), 1, 1),
         (torch.full_like(p, math.nan), torch.tensor([[1]]), None, torch.tensor([[0.0]]), torch.tensor([0.5]), 0, -1),
     ]
 
@@ -580,11 +588,60 @@ def test_offsets_beyond_32_bits():
 
 
 @pytest.mark.gpu
-def test_decode_step_in_graphs_and_on_streams():
+@pytest.mark.parametrize("code", CODES)
+def test_long_lines_are_shared_out_at_run_time(code):
+    """Enough blocks that warps fetch units as they finish: the same values every time, rows that nothing cuts and rows
+    that are cut many times."""
+
+    g = torch.Generator(DEV).manual_seed(2)
+    L, H, nb, U = 96, 4, 420, 2                                   # 161280 blocks, 63 for each of 2560 warps or fewer
+    codes = [torch.randint(-127, 128, (L, H, nb, U, 512), generator=g, device=DEV, dtype=torch.int8) for _ in range(2)]
+    if code != torch.int8:
+        codes = [torch.where((c & 0x7F) == 0x7F, 0, c).view(code) for c in codes]    # (no NaN code: 0x7f and 0xff)
+    scale = [torch.rand(L, H, nb, generator=g, device=DEV) * 0.02 for _ in range(2)]
+    held = [torch.zeros(L, H, 2, 64, 16, device=DEV, dtype=torch.float16) for _ in range(2)]
+    cache = D.KV8Cache(*codes, *scale, *held)
+    lengths = [64 * nb - 17 * l if l % 8 else 60 + l for l in range(L)]
+    q = torch.randn(L, H, 16, generator=g, device=DEV).half()
+    seg, n = seg_of([1] * L, DEV), i32(lengths, DEV)
+    runs = [ops.kv8_attention(q, cache, seg, n, 0.05) for _ in range(4)]
+    assert all(torch.equal(runs[0], r) for r in runs)
+    some = [0, 1, 8, 50, 95]
+    part = D.KV8Cache(*(c.view(torch.int8)[some].view(code) for c in codes), *(t[some] for t in scale + held))
+    check_attention(q[some], part, seg_of([1] * len(some)), [lengths[l] for l in some], 0.05, runs[0][some])
+
+
+@pytest.mark.gpu
+def test_first_calls_may_be_under_capture():
+    cache, _, _ = filled([70, 20], 2, 72, torch.float8_e4m3fn, torch.float16, device=DEV)
+    q = torch.randn(2, 2, 72, device=DEV).half()
+    seg, n = seg_of([1, 1], DEV), i32([70, 20], DEV)
+    wide = ops.kv8_cache(2, 2, 1 << 20, 104, DEV, torch.float8_e4m3fn, torch.float16)      # (units and a workspace)
+    k, q2 = torch.randn(2, 2, 104, device=DEV).half(), torch.randn(2, 6, 104, device=DEV).half()
+    p, x, d, u, w, lens = (t.to(DEV) for t in drafts(3, 2, 999, torch.float16, False, 5))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = ops.kv8_attention(q, cache, seg, n, 0.1)
+        ops.kv8_append(wide, k, k, seg, n * 0)
+        b = ops.kv8_attention(q2, wide, seg, n * 0 + 1, 0.1)
+        c = ops.verify_draft(p, x, d, u, w, lens)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(a, ops.kv8_attention(q, cache, seg, n, 0.1))
+    # one entry: its value, whatever the query
+    back = ops.kv8_read(wide, seg, n * 0, 2, dtype=torch.float16)[1]
+    assert torch.allclose(b.float(), back.repeat_interleave(3, 1).float(), rtol=2.0 ** -10)
+    assert all(torch.equal(i, j) for i, j in zip(c, ops.verify_draft(p, x, d, u, w, lens)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capacity", [1024, 300_000])             # by tasks; by units with a workspace
+def test_decode_step_in_graphs_and_on_streams(capacity):
     """Append and attention captured in two graphs that replay in turn, and on two streams at once."""
 
     def setup(seed):
-        cache, _, _ = filled([700, 90, 33], 2, 40, torch.int8, torch.bfloat16, seed=seed, capacity=1024, device=DEV)
+        cache, _, _ = filled([700, 90, 33], 2, 40, torch.int8, torch.bfloat16, seed=seed, capacity=capacity, device=DEV)
         g = torch.Generator().manual_seed(seed)
         q, k, v = (torch.randn(3, 2, 40, generator=g).bfloat16().to(DEV) for _ in range(3))
         return cache, q, k, v, seg_of([1, 1, 1], DEV), i32([700, 90, 33], DEV)
