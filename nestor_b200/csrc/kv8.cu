@@ -1237,10 +1237,10 @@ void with_types(int type, bool pair, int code, int U, F f) {
 }
 int unit_threads(int U) { return 32 * (U <= 8 ? U : (U + 1) / 2); }
 
-// Rows that one CTA looks through. Steps of few rows a list: one, since every row may begin a block. Longer runs: a block
-// each, or four where that still leaves two waves of CTAs (the search for the list and the first load are then paid once).
+// Rows that one CTA looks through: as many as a list brings, so that it finds one block or two, up to a block. Long runs
+// take four blocks where that still leaves two waves of CTAs (the search for the list and the first load are paid once).
 int chunk_of(int rows, int max_rows, int heads) {
-  if (max_rows <= 8) return 1;
+  if (max_rows < kBlock) return max_rows < 1 ? 1 : max_rows;
   return long(rows) * heads / (4 * kBlock) >= 2l * 12 * multiprocessors() ? 4 * kBlock : kBlock;
 }
 
