@@ -334,11 +334,26 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
   const int end = max(0, min(p.seg[c.L], p.rows));
   T* dst[2] = {reinterpret_cast<T*>(p.dst[0]) + long(h) * D, reinterpret_cast<T*>(p.dst[1]) + long(h) * D};
   const long rs = long(c.H) * D;
+  // (rows are as far apart as the head of one row is wide or a multiple of it, so they share its alignment)
+  const bool by16 = D * sizeof(T) % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.dst[0]) | reinterpret_cast<uintptr_t>(p.dst[1])) & 15) == 0;
   auto zeros = [&](int a, int b) {
-    for (int i = threadIdx.x; i < (b - a) * D; i += blockDim.x) {
-      const int e = i / D;
-      const long at = long(a + e) * rs + (i - e * D);
-      dst[0][at] = dst[1][at] = from_f<T>(0.f);
+    if (by16) {
+      const int n = D * int(sizeof(T)) / 16;
+      for (int i = threadIdx.x; i < (b - a) * n; i += blockDim.x) {
+        const int e = i / n;
+        const long at = long(a + e) * rs;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) reinterpret_cast<uint4*>(dst[kv] + at)[i - e * n] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      return;
+    }
+    const int n = (D + 1) / 2;
+    for (int i = threadIdx.x; i < (b - a) * n; i += blockDim.x) {
+      const int e = i / n, d = 2 * (i - e * n);
+      Two<T> z;
+      make_zero(z);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) store_two<T, PAIR>(dst[kv] + long(a + e) * rs + d, z, d + 1 < D);
     }
   };
   int r = int(blockIdx.x / c.H) * chunk;

@@ -116,6 +116,7 @@ def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype
 
 
 LOG2E = math.log2(math.e)
+_sizes: dict = {}          # bytes of workspace for a shape (a function of the shape and the device alone)
 
 
 def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor, scale: float, max_rows: int = 1,
@@ -132,12 +133,14 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     o_row, o_head, _ = out.stride()
     group, max_rows = q.shape[1] // cache.heads, min(max_rows, rows)
     L = _L()
-    index = cache.device.index
-    if _device() == index:
-        size = L.nb_kv8_attention_workspace(cache.lists, cache.heads, cache.blocks, cache.head_dim, rows, max_rows, group)
-    else:
-        with torch.cuda.device(index):
-            size = L.nb_kv8_attention_workspace(cache.lists, cache.heads, cache.blocks, cache.head_dim, rows, max_rows, group)
+    key = (cache.lists, cache.heads, cache.blocks, cache.head_dim, rows, max_rows, group)
+    size = _sizes.get((cache.device.index, key))
+    if size is None:
+        with torch.cuda.device(cache.device):
+            size = L.nb_kv8_attention_workspace(*key)
+        if len(_sizes) >= 4096:
+            _sizes.clear()
+        _sizes[cache.device.index, key] = size
     # (allocated for this call on this stream: two streams, or two captured graphs, never share it)
     ws = lengths.new_empty(-(-size // 4)) if size else None
     a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(), lengths.data_ptr(), rows,

@@ -59,11 +59,15 @@ class KV8Cache:
             raise ValueError(f"cache of {L} lists x {H} heads x {nb} blocks x {U} units for head_dim {D}: needs at least one of "
                              f"each, head_dim in 1..{MAX_HEAD_DIM} and ceil(head_dim / 8) units")
         device = k_codes.device
-        codes, scales, kept = (L, H, nb, U, 512), (L, H, nb), (L, H, 2, BLOCK, D)
-        for t, want in ((k_codes, codes), (v_codes, codes), (k_scale, scales), (v_scale, scales), (k_open, kept), (v_open, kept)):
-            if t.shape != want or t.device != device or not t.is_contiguous():
-                raise ValueError(f"cache tensors must be contiguous, on one device and of matching shapes: got {tuple(t.shape)} on {t.device}, "
-                                 f"expected {want} on {device}")
+        scales = (L, H, nb)
+        if not (shape == (L, H, nb, U, 512) == v_codes.shape and k_scale.shape == scales == v_scale.shape
+                and held == (L, H, 2, BLOCK, D) == v_open.shape):
+            raise ValueError(f"cache tensors of unlike shapes: codes {tuple(shape)} and {tuple(v_codes.shape)}, scales {tuple(k_scale.shape)} and "
+                             f"{tuple(v_scale.shape)}, originals {tuple(held)} and {tuple(v_open.shape)}")
+        tensors = (k_codes, v_codes, k_scale, v_scale, k_open, v_open)
+        for t in tensors:
+            if t.device != device or not t.is_contiguous():
+                raise ValueError(f"cache tensors must be contiguous and on one device, {device}; got {tuple(t.shape)} with strides {t.stride()} on {t.device}")
         if k_codes.data_ptr() % 16 or v_codes.data_ptr() % 16:
             raise ValueError("cache codes must begin on a 16-byte boundary")
         if nb * BLOCK >= 2 ** 31:

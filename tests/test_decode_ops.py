@@ -186,7 +186,7 @@ def test_refusals():
         ops.kv8_cache(1, 1, 1, 8, dtype=torch.uint8)
     with pytest.raises(ValueError, match="head_dim"):
         ops.kv8_cache(1, 1, 1, 129)
-    with pytest.raises(ValueError, match="shapes"):
+    with pytest.raises(ValueError, match="unlike shapes"):
         ops.KV8Cache(cache.k_codes, cache.v_codes, cache.k_scale, cache.v_scale[:1], cache.k_open, cache.v_open)
     with pytest.raises(AttributeError, match="fixed"):
         cache.k_scale = cache.v_scale
