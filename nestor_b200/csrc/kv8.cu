@@ -8,9 +8,9 @@
 // a warp need them as the 16-bit A operand of mma.m16n8k16 (g = lane / 4, t = lane % 4, bytes (m, h, i)):
 //   keys   : entry 16m + 8h + g,       dim 8u + 2t + i      (rows = entries, reduction = dims)
 //   values : entry 16m + 8h + 2t + i,  dim 8u + g           (rows = dims, reduction = entries)
-// A unit is therefore one fully coalesced 16-byte load per lane straight into registers: the attention stages nothing
-// in shared memory, has no bank conflicts and no barriers, and a (list, head) is one contiguous stream. Head dims need
-// rounding up to a multiple of 8 only.
+// A unit is therefore one 16-byte load per lane, coalesced in memory and without bank conflicts in shared memory, that
+// needs no shuffle before the product, and the keys (the values) of a (list, head) are one contiguous stream. Head dims
+// need rounding up to a multiple of 8 only; codes of dims past the head are zero.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -63,8 +63,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __
 //
 // A warp owns a unit (two of them above 8): its lanes load the pairs of dims of eight entries that they hold in the keys'
 // layout, so nothing passes through shared memory but the warps' maxima. The values' layout is the transpose of each
-// 8 x 8 tile: their codes go through movmatrix as 16-bit numbers. About 6 instructions an element; through a tile in
-// shared memory it was 20, and those, not HBM, were the bound.
+// 8 x 8 tile: their codes go through movmatrix as 16-bit numbers. Instructions, not HBM, are the bound: about 14 an
+// element, half of what a tile in shared memory took (197k rows x 3 heads x 40 in bf16: 55 us instead of 108; HBM alone
+// would take 22).
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -414,12 +415,12 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // Both code types convert to fp16 without rounding. One pass over the entries with the running maximum and sum of the
 // softmax; a block's scales multiply its scores and its partial output in fp32.
 //
-// What bounds it: one query reads 2 bytes of cache for 4 flops, so HBM does; the tensor pipe is used because a column
-// tile of 8 costs no more than one query, and because the conversion (1.25 instructions a code) is then the largest
-// part of a warp's work.
+// What bounds it: one query reads 2 bytes of cache for 4 flops, so HBM does (192 lists of 6144 to 12288 entries x 5 x 40,
+// int8, 0.71 GB: 124 us, 5.7 TB/s with both launches). The tensor pipe is used because a column tile of 8 costs no more
+// than one query; the conversion (0.75 instructions a code) is then the largest part of a warp's work.
 //
-// Precision. q is scaled per column by a power of two into [1, 2) and rounded to fp16 (exact for bf16 and fp16
-// queries, two fp16 numbers for fp32 ones); probabilities are multiplied by 2^7 before their rounding to fp16, so that
+// Precision. q is scaled per column by a power of two, into [1, 2) or, where the products carry a factor 2^-24, into
+// [2^14, 2^15), and rounded to fp16 (exact for bf16 and fp16 queries, two fp16 numbers for fp32 ones); probabilities are multiplied by 2^7 before their rounding to fp16, so that
 // weights down to 2^-21 of the largest keep 11 bits, and the sum of the softmax adds the rounded weights. Where the
 // output has more than bf16's 8 bits, probabilities are two fp16 numbers as well, which keeps 22.
 //
@@ -427,13 +428,13 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // takes a task, its warps take equal runs of the blocks and join their results in shared memory. Otherwise all blocks of
 // all tasks form one line that is cut into units, a warp each. A warp that owns a whole task writes its output; pieces of
 // a task that is cut go to a workspace and `attn_join` adds them in order, so results do not depend on the schedule. Short
-// lines: one unit a warp. Long ones (32 blocks a warp and more): five sixths in one unit a warp, the rest in as many
-// smaller ones that the warps fetch as they finish, because equal shares end up to a quarter apart (0.7 GB: the last warp
-// at 128 us instead of 117). A unit costs some 3 us beside its blocks (queries, scales, its piece) and twice the units cost
-// the join 4 us: a line of 20 blocks a warp took 92 us so and takes 80 without, and more and smaller units lost as well.
+// lines: one unit a warp, of two blocks at least. Long ones (32 blocks a warp and more): five sixths in one unit a warp,
+// the rest in as many smaller ones that the warps fetch as they finish, because equal shares end up to a quarter apart
+// (0.7 GB: the last warp at 128 us instead of 117). A unit costs some 3 us beside its blocks (queries, scales, its piece)
+// and twice the units cost the join 4 us: a line of 20 blocks a warp took 92 us so and takes 80 without, and more and
+// smaller units lost as well.
 constexpr float kShift = 7.f;        // log2 of the factor on the probabilities
 constexpr float kSlack = 8.f;        // how far (log2) a score may pass the running maximum; 2^(kShift + kSlack) fits fp16
-constexpr int kJoin = 4;             // warps of a CTA of attn_join
 constexpr int kMaxLists = 1024;      // lists in one launch (their prefix sums stay in shared memory)
 
 struct Attn {
@@ -457,7 +458,7 @@ struct Cuts {
       units = (1 + kShares) * workers;
       head = t - t / 6;
     } else {
-      units = workers = int(max(1l, min(long(k.workers), t)));
+      units = workers = int(max(1l, min(long(k.workers), t / 2)));
       head = t;
     }
   }
@@ -1103,15 +1104,16 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   }
 }
 
-// Adds the pieces of each (row, query head) whose task was cut, in their order. TEAM warps share an item: 4 where there
-// are few items (their tasks are cut into many pieces then), else 1. Rows behind the last list become zeros when
+// Adds the pieces of each (row, query head) whose task was cut, in their order. TEAM warps share an item: the fewer items,
+// the more pieces their tasks are cut into, so 16, 4 or 1. Rows behind the last list become zeros when
 // `zero_tail` is set. What it is bound by is the chain of loads behind the main kernel's end: the item's cut, then all
 // pieces at once.
 template <int TEAM>
-__global__ void __launch_bounds__(kJoin * 32) attn_join(const Attn k, int cols) {
-  __shared__ float tops[kJoin], sums[kJoin], acc_s[kJoin][128];
+__global__ void __launch_bounds__((TEAM < 4 ? 4 : TEAM) * 32) attn_join(const Attn k, int cols) {
+  constexpr int WARPS = TEAM < 4 ? 4 : TEAM;
+  __shared__ float tops[WARPS], sums[WARPS], acc_s[WARPS][128];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, member = warp % TEAM, heads = k.c.H * k.a.group;
-  const long item = blockIdx.x * long(kJoin / TEAM) + warp / TEAM;
+  const long item = blockIdx.x * long(WARPS / TEAM) + warp / TEAM;
   const int row = int(item / heads), head = int(item - long(row) * heads);
   const int L = k.c.L, D = k.c.D, width = 8 * k.c.U + 2, seg_begin = k.a.seg[0], seg_end = k.a.seg[L];
   const bool exists = item < long(k.a.rows) * heads;
@@ -1155,14 +1157,15 @@ __global__ void __launch_bounds__(kJoin * 32) attn_join(const Attn k, int cols) 
     for (int i = 0; i < TEAM; ++i) top = fmaxf(top, tops[i]);
     float x = 0.f;
     sum = 0.f;
-    const int d = threadIdx.x;         // (128 threads, at most 128 dims)
+    const int d = threadIdx.x;         // (at least 128 threads, at most 128 dims)
+    if (d >= D) return;
 #pragma unroll
     for (int i = 0; i < TEAM; ++i) {
       const float f = tops[i] == top ? 1.f : ex2(tops[i] - top);
       sum += f * sums[i];
       x += f * acc_s[i][d];
     }
-    if (d < D) store_any(k.a.out, at + d, k.a.q_type, sum == 0.f ? 0.f : x / sum);
+    store_any(k.a.out, at + d, k.a.q_type, sum == 0.f ? 0.f : x / sum);
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -1252,10 +1255,12 @@ void with_types(int type, bool pair, int code, int U, F f) {
 }
 int unit_threads(int U) { return 32 * (U <= 8 ? U : (U + 1) / 2); }
 
-// Rows that one CTA looks through: as many as a list brings, so that it finds one block or two, up to a block. Long runs
-// take four blocks where that still leaves two waves of CTAs (the search for the list and the first load are paid once).
-int chunk_of(int rows, int max_rows, int heads) {
-  if (max_rows < kBlock) return max_rows < 1 ? 1 : max_rows;
+// Rows that one CTA looks through: as many as a list brings on average (at most `max_rows`), so that it finds one block or
+// two, up to a block. Long runs take four blocks where that still leaves two waves of CTAs (the search for the list and
+// the first load are paid once).
+int chunk_of(int rows, int max_rows, int heads, int lists) {
+  const int each = std::max(1, std::min((rows + lists - 1) / lists, max_rows));
+  if (each < kBlock) return each;
   return long(rows) * heads / (4 * kBlock) >= 2l * 12 * multiprocessors() ? 4 * kBlock : kBlock;
 }
 
@@ -1274,7 +1279,7 @@ int nb_kv8_append(const nb_kv8_cache* c, const nb_kv8_rows* p, cudaStream_t st) 
   const long strides[4] = {p->row_stride[0], p->row_stride[1], p->head_stride[0], p->head_stride[1]};
   const void* ptrs[4] = {p->src[0], p->src[1], c->open[0], c->open[1]};
   const bool pair = pairs(c->D, c->type == 2 ? 4 : 2, strides, 4, ptrs, 4);
-  const int chunk = chunk_of(p->rows, p->max_rows, c->H);
+  const int chunk = chunk_of(p->rows, p->max_rows, c->H, c->L);
   const long grid = (long(p->rows) + chunk - 1) / chunk * c->H;
   if (grid > 0x7fffffffl) return -1;
   with_types(c->type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
@@ -1300,7 +1305,7 @@ int nb_kv8_read(const nb_kv8_cache* c, const nb_kv8_rows* p, int type, cudaStrea
   if (p->rows == 0) return 0;
   const void* ptrs[2] = {p->dst[0], p->dst[1]};
   const bool pair = pairs(c->D, type == 2 ? 4 : 2, nullptr, 0, ptrs, 2);
-  const int chunk = chunk_of(p->rows, p->max_rows, c->H);
+  const int chunk = chunk_of(p->rows, p->max_rows, c->H, c->L);
   const long grid = (long(p->rows) + chunk - 1) / chunk * c->H;
   if (grid > 0x7fffffffl) return -1;
   with_types(type, pair, c->code, c->U, [&](auto t, auto v, auto k, auto n) {
@@ -1346,7 +1351,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
   using namespace nbk;
   if (bad_cache(c) || a->rows < 0 || a->group < 1 || a->max_rows < 1) return -1;
   // (a list's tasks are counted in 32 bits)
-  if (long(c->H) * ((long(a->rows) * a->group + 7) / 8) * c->nb > 0x7fffffffl) return -3;
+  if (long(a->rows) * a->group > (1l << 30) || long(c->H) * ((long(a->rows) * a->group + 7) / 8) * c->nb > 0x7fffffffl) return -3;
   if (a->rows == 0) return 0;
   const Plan plan = plan_of(c->L, c->H, c->nb, c->D, a->rows, a->max_rows, a->group);
   if (plan.bytes > ws_bytes) return -2;
@@ -1388,17 +1393,19 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
     k.workers = grid * plan.warps;
     fn<<<grid, plan.warps * 32, smem, st>>>(k);
     if ((rc = cudaGetLastError()) != cudaSuccess) return int(rc);
-    const bool teams = items <= 32l * plan.sms;
+    const int team = items <= 2l * plan.sms ? 16 : items <= 32l * plan.sms ? 4 : 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(teams ? items : (items + kJoin - 1) / kJoin));
-    cfg.blockDim = dim3(kJoin * 32);
+    cfg.gridDim = dim3(unsigned(team > 1 ? items : (items + 3) / 4));
+    cfg.blockDim = dim3(team > 4 ? team * 32 : 128);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    rc = teams ? cudaLaunchKernelEx(&cfg, attn_join<kJoin>, (const Attn)k, plan.cols) : cudaLaunchKernelEx(&cfg, attn_join<1>, (const Attn)k, plan.cols);
+    using Join = void (*)(const Attn, int);
+    const Join join = team == 16 ? attn_join<16> : team == 4 ? attn_join<4> : attn_join<1>;
+    rc = cudaLaunchKernelEx(&cfg, join, k, plan.cols);
     if (rc != cudaSuccess) return int(rc);
   }
   return 0;

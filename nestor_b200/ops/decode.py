@@ -32,7 +32,8 @@ class KV8Cache:
 
     Attributes (fixed once built):
         k_codes, v_codes: ``[L, H, blocks, ceil(head_dim / 8), 512]`` int8 or float8_e4m3fn. A block's codes are units of
-            8 head dims x 64 entries in the order of the kernels' matrix fragments (:func:`code_positions`).
+            8 head dims x 64 entries in the order of the kernels' matrix fragments (:func:`code_positions`); codes of dims
+            past ``head_dim`` are zero.
         k_scale, v_scale: ``[L, H, blocks]`` fp32.
         k_open, v_open: ``[L, H, 2, 64, head_dim]`` originals of the youngest two blocks (block ``b`` in slot ``b % 2``),
             in the dtype of the rows that are appended (bf16, fp16 or fp32).
@@ -157,7 +158,8 @@ def check_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tens
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"kv8_attention: scale must be positive and finite, got {scale}")
     check_count("kv8_attention", shape[0], max_rows)
-    if cache.heads * -(-shape[0] * (shape[1] // cache.heads) // 8) * cache.blocks >= 2 ** 31:
+    columns = shape[0] * (shape[1] // cache.heads)
+    if columns > 2 ** 30 or cache.heads * -(-columns // 8) * cache.blocks >= 2 ** 31:
         raise ValueError(f"kv8_attention: {shape[0]} rows x {shape[1]} heads over {cache.blocks} blocks are too many for one call: pass them in parts")
     if out is not None:
         step = out.stride()

@@ -583,8 +583,9 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(back[1], ops.kv8_read(small, seg_of([140], DEV), i32([0], DEV), 140)[1])
     q = torch.randn(1, H, hd, generator=g).bfloat16().to(DEV)
     a = ops.kv8_attention(q, cache, seg_of([0] * (L - 1) + [1], DEV), i32([0] * (L - 1) + [140], DEV), 0.125)
-    b = ops.kv8_attention(q, small, seg_of([1], DEV), i32([140], DEV), 0.125)
-    assert torch.equal(a, b)
+    # (the two capacities divide the work differently, so the sums may differ in their last bits: both have the bound)
+    check_attention(q, small, seg_of([1], DEV), [140], 0.125, a)
+    check_attention(q, small, seg_of([1], DEV), [140], 0.125, ops.kv8_attention(q, small, seg_of([1], DEV), i32([140], DEV), 0.125))
 
 
 @pytest.mark.gpu
