@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 SRC = Path(__file__).resolve().parent
@@ -64,27 +65,32 @@ def _build_locked(verbose: bool, force: bool, checked: bool) -> Path:
     cc = nvcc()
     if cc is None:
         raise RuntimeError("nvcc not found: cannot build the sm_100a kernel library")
-    objs, rebuilt = [], False
     extra = ["-DNESTOR_BOUNDS_CHECK"] if checked else []
     kind = "chk" if checked else ""
-    for cu in sorted(SRC.glob("*.cu")):
+
+    def compiled(cu: Path) -> tuple[Path, bool]:
         obj = OUT / f"{cu.stem}{kind}.{_digest(cu)}.o"
-        if force or not obj.is_file():
-            for old in OUT.glob(f"{cu.stem}{kind}.*.o"):
-                old.unlink(missing_ok=True)
-            tmp = obj.with_suffix(f".{os.getpid()}.tmp")
-            cmd = [cc, *FLAGS, *extra, "-c", str(cu), "-o", str(tmp)]
-            res = subprocess.run(cmd, capture_output=True, text=True)
-            if verbose or res.returncode:
-                sys.stderr.write(res.stdout + res.stderr)
-            if res.returncode:
-                tmp.unlink(missing_ok=True)
-                raise RuntimeError(f"nvcc failed on {cu.name}")
-            tmp.replace(obj)
-            if not checked:
-                (OUT / f"{cu.stem}.ptxas.txt").write_text(res.stderr)
-            rebuilt = True
-        objs.append(obj)
+        if not force and obj.is_file():
+            return obj, False
+        for old in OUT.glob(f"{cu.stem}{kind}.*.o"):
+            old.unlink(missing_ok=True)
+        tmp = obj.with_suffix(f".{os.getpid()}.tmp")
+        cmd = [cc, *FLAGS, *extra, "-c", str(cu), "-o", str(tmp)]
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or res.returncode:
+            sys.stderr.write(res.stdout + res.stderr)
+        if res.returncode:
+            tmp.unlink(missing_ok=True)
+            raise RuntimeError(f"nvcc failed on {cu.name}")
+        tmp.replace(obj)
+        if not checked:
+            (OUT / f"{cu.stem}.ptxas.txt").write_text(res.stderr)
+        return obj, True
+
+    # the sources side by side: one of them takes as long as all others together
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        done = list(pool.map(compiled, sorted(SRC.glob("*.cu"))))
+    objs, rebuilt = [obj for obj, _ in done], any(new for _, new in done)
     lib = CHECKED_LIB if checked else LIB
     if rebuilt or not lib.is_file():
         tmp = lib.with_suffix(f".{os.getpid()}.tmp")
