@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // softmax; a block's scales multiply its scores and its partial output in fp32.
 //
 // What bounds it: one query reads 2 bytes of cache for 4 flops, so HBM does (192 lists of 6144 to 12288 entries x 5 x 40,
-// int8, 0.71 GB: 124 us, 5.7 TB/s with both launches). The tensor pipe is used because a column tile of 8 costs no more
+// int8, 0.71 GB: 125 us, 5.7 TB/s with both launches). The tensor pipe is used because a column tile of 8 costs no more
 // than one query; the conversion (0.75 instructions a code) is then the largest part of a warp's work.
 //
 // Precision. q is scaled per column by a power of two, into [1, 2) or, where the products carry a factor 2^-24, into

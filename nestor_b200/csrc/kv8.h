@@ -1,4 +1,4 @@
-// Argument blocks of the 8-bit key/value cache entry points (mirrored by ctypes structures in ops/decode.py).
+// Argument blocks of the 8-bit key/value cache entry points (mirrored by ctypes structures in ops/cuda_decode.py).
 #pragma once
 #include <cuda_runtime.h>
 

@@ -227,7 +227,9 @@ extern "C" int nb_verify_draft(const nb_verify_args* a, cudaStream_t st) {
   if (a->B == 0) return 0;
   // Spans that keep the sums within their 8 KB, and no more CTAs a row than there are spans for half of their warps or than
   // fit the GPU at once: a second wave would wait for its first loads while the first one's end idles (256 rows of
-  // 100263: 45 us in one wave, 48 to 63 in more). Many rows take CTAs of 4 warps instead of 8, which spread evenly.
+  // 100263 in fp32, CTAs a row x warps: 36.4 us for 4 x 4, the whole of one wave; 40.3 for 8 x 4, 60.5 for 1 x 4). Many
+  // rows take CTAs of 4 warps instead of 8, which spread evenly (1024 rows of 50257: 54.0 us for 1 x 4, 57.1 for 1 x 8);
+  // few rows take 8 (64 rows of 100263: 11.9 us against 12.5).
   int span = 512;
   while ((a->V + span - 1) / span > kMaxSpans) span *= 2;
   int dev = 0, sms = 148;

@@ -1,4 +1,4 @@
-// Argument block of nb_verify_draft (mirrored by a ctypes structure in ops/decode.py).
+// Argument block of nb_verify_draft (mirrored by a ctypes structure in ops/cuda_decode.py).
 #pragma once
 #include <cuda_runtime.h>
 

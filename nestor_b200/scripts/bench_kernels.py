@@ -196,8 +196,8 @@ def case_gather(reps: int, small: bool = False) -> None:
 
 @torch.no_grad()
 def case_decode(reps: int) -> None:
-    """One layer of a decode step of 64 sequences over 12288 entries a list (the first block's 3 of 8 columns), a prompt of
-    8 x 4096 tokens entering its lists, and the verification of 4 drafted tokens of 256 sequences."""
+    """One layer of a decode step of 64 sequences over 12288 entries a list (the first block's 3 of 8 columns), 48 lists of
+    4096 rows entered and read back, and the verification of 4 drafted tokens of 256 sequences."""
 
     from nestor_b200 import ops
     _, bw, src = peaks()
@@ -218,10 +218,10 @@ def case_decode(reps: int) -> None:
         report(f"attention, 192 rows x {n}, {code}", timed(lambda: ops.kv8_attention(q, cache, seg, start + 1, 1 / hd), reps),
                192 * H * n * (2 * hd + 8 / 64))
         del cache, fill
-    rows = 8 * 6 * 4096
-    cache = ops.kv8_cache(64, 3, 4096, hd, "cuda")
-    seg = torch.arange(0, rows + 1, rows // 64, dtype=torch.int32, device="cuda")
-    zero = torch.zeros(64, dtype=torch.int32, device="cuda")
+    rows = 48 * 4096
+    cache = ops.kv8_cache(48, 3, 4096, hd, "cuda")
+    seg = torch.arange(0, rows + 1, 4096, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(48, dtype=torch.int32, device="cuda")
     k, v = (torch.randn(rows, 3, hd, device="cuda").to(BF) for _ in range(2))
     report(f"append, {rows} rows", timed(lambda: ops.kv8_append(cache, k, v, seg, zero, max_rows=4096), reps), rows * 3 * hd * 2 * 3)
     report(f"read, {rows} rows", timed(lambda: ops.kv8_read(cache, seg, zero, rows, dtype=BF), reps), rows * 3 * hd * 2 * 3)
