@@ -473,6 +473,8 @@ class NestorKVCache:
         if bool((dropped < 0).any()) or bool((dropped > held).any()):
             raise ValueError("only tokens that the decode state remembers can be taken back (the newest "
                              f"{self.TAKE_BACK} of a sequence, each once)")
+        if self.recent[0] is None:
+            return                                                           # (nothing was fed, nothing is taken back)
         for i, (rec, layers) in enumerate(zip(self.recent, self.blocks)):
             R, k = rec.shape[1:]
             back = torch.arange(R, device=rec.device).unsqueeze(0) - dropped.unsqueeze(1)          # where slot j moves from

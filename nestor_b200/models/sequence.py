@@ -327,12 +327,14 @@ class SequenceModel(nn.Module):
 
     @torch.no_grad()
     def decode_step(self, ids: Tensor, cache, pos: Tensor | None = None) -> Tensor:
-        """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` (``cache`` is advanced). Several tokens
-        ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n`` single steps
-        otherwise."""
+        """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` or ``[B, 1]`` (``cache`` is advanced).
+        Several tokens ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n``
+        single steps otherwise."""
 
         if ids.shape[0] != cache.batch:
             raise ValueError(f"the cache decodes {cache.batch} sequences, got tokens for {ids.shape[0]}")
+        if ids.dim() == 2 and ids.shape[1] == 1:
+            ids, pos = ids[:, 0], None if pos is None else pos.reshape(-1)
         if ids.dim() == 2:
             if not cache.eight_bit:
                 steps = [self.decode_step(ids[:, t], cache, None if pos is None else pos[:, t]) for t in range(ids.shape[1])]
@@ -432,6 +434,8 @@ class SequenceModel(nn.Module):
             u = torch.rand(B, n, generator=generator, device=dev)
             w = torch.rand(B, generator=generator, device=dev)
             accepted, token = ops.verify_draft(target, x, q, u, w)
+            if bool((token < 0).any()):
+                raise RuntimeError("the model's probabilities leave no token to draw (its logits are not finite)")
             accepted, token = accepted.long(), token.to(prompt.dtype)
             # sequences that have their tokens wait for the others: they keep nothing of the round
             live = end < S0 + max_new_tokens

@@ -80,6 +80,10 @@ class KV8Cache:
     def __setattr__(self, name: str, value) -> None:
         raise AttributeError(f"the {name} of a KV8Cache is fixed (its kernels keep an argument block of it); build another one")
 
+    def __reduce__(self):
+        # (copies and pickles are built from the tensors, so they say where their own tensors are)
+        return KV8Cache, (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_open, self.v_open)
+
 
 def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None, dtype: torch.dtype = torch.int8,
               open_dtype: torch.dtype = torch.bfloat16) -> KV8Cache:
@@ -147,7 +151,7 @@ def check_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dty
 
 
 def check_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor, scale: float, max_rows: int, out: Tensor | None) -> None:
-    check_no_grad("kv8_attention", q)
+    check_no_grad("kv8_attention", q, out)
     shape = q.shape
     if (len(shape) != 3 or shape[2] != cache.head_dim or shape[1] < 1 or shape[1] % cache.heads or q.dtype not in FLOATS
             or q.device != cache.device):
@@ -325,8 +329,9 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     head ``h * H // Hq``). ``lengths [L]`` counts the entries of each list with the new rows' own among them, so row
     ``a`` of the ``n`` rows of list ``l`` sees the first ``lengths[l] - (n - 1 - a)`` entries. Softmax of
     ``scale * q . k`` in fp32, output in ``q.dtype``; a row that sees nothing gives zeros. Rows behind ``seg_start[-1]``
-    are left as they are in ``out`` and are zeros without it. ``max_rows`` (how many rows a list brings at most) only
-    steers speed. ``lengths`` beyond the capacity count as the capacity and are reported like in :func:`kv8_append`.
+    are left as they are in ``out`` (which may be ``q`` itself, but must not overlap it otherwise) and are zeros without
+    it. ``max_rows`` (how many rows a list brings at most) only steers speed. ``lengths`` beyond the capacity count as the
+    capacity and are reported like in :func:`kv8_append`.
     """
 
     check_attention(q, cache, seg_start, lengths, scale, max_rows, out)
@@ -363,7 +368,7 @@ def verify_draft(target_probs: Tensor, draft_tokens: Tensor, draft_probs: Tensor
     Token ``i`` is accepted while ``u_i q_i(x_i) < p_i(x_i)`` (fp32 product). With ``a`` accepted, the next token is the
     lowest ``j`` with ``r_0 + .. + r_j > w * sum(r)``, summed in 64 bits, where ``r = p_len`` if all were accepted and
     otherwise ``r = max(p_a - q_a, 0)`` (``p_a`` without ``x_a`` where there are no ``draft_probs``), or ``p_a`` if that
-    leaves nothing. ``-1`` if ``p_a`` has no mass either. Values that are not above ``2^-126`` (NaN too) count as zero,
+    leaves nothing. ``-1`` if ``p_a`` has no mass either. Values below ``2^-126`` and NaN count as zero,
     tokens outside the vocabulary as refused.
     """
 

@@ -109,12 +109,35 @@ def test_tokens_are_taken_back_sequence_by_sequence(eight_bit, tiny_scale, monke
     assert cache.positions.tolist() == [0, 9, 15]
     step = m.decode_step(torch.stack([ids[0, :1], ids[1, 9:10], ids[2, 15:16]]), cache)
     for b, t in enumerate((0, 9, 15)):
-        assert torch.allclose(step[b, 0], full[b, t], atol=2e-4, rtol=1e-4)
+        assert torch.allclose(step[b], full[b, t], atol=2e-4, rtol=1e-4)
     for bad in ([2, 0, 0], [-1, 0, 0]):
         with pytest.raises(ValueError, match="taken back"):
             cache.rollback(torch.tensor(bad))
     with pytest.raises(ValueError, match="one entry per sequence"):
         cache.rollback(torch.tensor([0, 0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int8])
+def test_steps_of_one_token_and_of_none(dtype, tiny_scale):
+    m = tiny(tiny_scale, "nestor", 1)
+    ids = torch.randint(0, 100263, (2, 3))
+    flat, column = (m.init_kv_cache(2, 8, dtype=dtype) for _ in range(2))
+    flat.rollback(torch.tensor([0, 0]))              # nothing was fed yet
+    with pytest.raises(ValueError, match="taken back"):
+        flat.rollback(torch.tensor([1, 0]))
+    for t in range(3):
+        a, b = m.decode_step(ids[:, t], flat), m.decode_step(ids[:, t : t + 1], column, torch.full((2, 1), t))
+        assert a.shape == (2, 100263) and torch.equal(a, b)
+    assert m.decode_step(ids[:, :0], flat).shape == (2, 0, 100263) and flat.length == 3
+
+
+def test_logits_without_a_number_end_the_drafted_decoding(tiny_scale):
+    m, draft = tiny(tiny_scale, "moe", 5), tiny(tiny_scale, "dense", 6)
+    prompt = torch.randint(0, 100263, (2, 4))
+    with torch.no_grad():
+        m.head.weight.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="no token to draw"):
+        m.generate(prompt, 4, 0.8, torch.Generator().manual_seed(0), torch.int8, draft, 3)
 
 
 @pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])

@@ -1,6 +1,8 @@
 """The decoding ops: 8-bit key/value cache (append, truncate, read, attention) and verification of drafted tokens."""
 
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -231,6 +233,39 @@ def test_refusals():
         ops.kv8_attention(row, cache, seg, i32([0, 129]), 1.0)
     with pytest.raises(RuntimeError, match="no_grad"):
         ops.kv8_attention(row.clone().requires_grad_(), cache, seg, start, 1.0)
+    with pytest.raises(RuntimeError, match="no_grad"):
+        ops.kv8_attention(row, cache, seg, start, 1.0, out=row.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_copies_of_a_cache_go_their_own_way(device):
+    cache = ops.kv8_cache(2, 3, 100, 16, device)
+    rows = [torch.randn(4, 3, 16, device=device).bfloat16() for _ in range(2)]
+    seg, at = torch.tensor([0, 2, 4], dtype=torch.int32, device=device), torch.zeros(2, dtype=torch.int32, device=device)
+    ops.kv8_append(cache, *rows, seg, at, max_rows=2)
+    twins = copy.deepcopy(cache), pickle.loads(pickle.dumps(cache))
+    before = [t.clone() for t in ops.kv8_read(cache, seg, at, 4)]
+    ops.kv8_append(cache, -rows[0], -rows[1], seg, at, max_rows=2)
+    for twin in twins:
+        assert twin.k_codes.data_ptr() != cache.k_codes.data_ptr() and twin.device == cache.device
+        for x, y, z in zip(before, ops.kv8_read(twin, seg, at, 4), ops.kv8_read(cache, seg, at, 4)):
+            assert torch.equal(x, y) and torch.equal(x, -z)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("capacity", [1024, 300_000])             # by tasks; by units with a workspace
+def test_attention_into_its_own_queries(capacity):
+    n = 700
+    cache = ops.kv8_cache(2, 2, capacity, 40, "cuda")
+    seg = torch.tensor([0, n, 2 * n], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(2 * n, 2, 40, device="cuda").bfloat16() for _ in range(2))
+    ops.kv8_append(cache, k, v, seg, torch.zeros(2, dtype=torch.int32, device="cuda"), max_rows=n)
+    q = torch.randn(6, 4, 40, device="cuda").bfloat16()
+    few, lengths = torch.tensor([0, 3, 5], dtype=torch.int32, device="cuda"), torch.tensor([n, n - 60], dtype=torch.int32, device="cuda")
+    want = ops.kv8_attention(q, cache, few, lengths, 1 / 40, max_rows=3)
+    own = q.clone()
+    assert ops.kv8_attention(own, cache, few, lengths, 1 / 40, max_rows=3, out=own) is own
+    assert torch.equal(own[:5], want[:5]) and torch.equal(own[5:], q[5:])
 
 
 def test_argument_blocks_match_the_built_library():
