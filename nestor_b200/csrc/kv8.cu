@@ -445,6 +445,7 @@ struct Attn {
   int2* cut;          // [rows][query heads]: of the item's task the first unit; the number of pieces * 16 + the item's column
   float* ws;          // pieces: slot 2u for a task that unit u continues, 2u + 1 for one that it begins
   int workers, dynamic, by_task;
+  unsigned polls;     // looks at a copy's barrier before the wait for it gives up
 };
 
 constexpr int kShares = 1;           // small units for each warp of a long line
@@ -719,24 +720,20 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   int slot = 0;
   uint32_t parity = 0;
   const uint32_t ring_at = nb::smem_u32(ring) + lane * 16;
-  // Waits for the copy in `slot`. A copy that never lands ends the warp: the status word is set, whatever is still in
-  // flight gets the same bounded time, and the warp's rows keep what they held.
+  // Waits for the copy in `slot`. Where the wait gives up, the status word is set, whatever is still in flight gets a
+  // bounded time of its own, and the warp goes on at `gave_up`.
   auto landed = [&]() {
-    if (!__all_sync(0xffffffffu, nb::mbar_try_wait(&bars[warp][slot], parity))) {
-      uint32_t i = 0;
-      while (!__all_sync(0xffffffffu, nb::mbar_try_wait(&bars[warp][slot], parity)))
-        if (++i == nb::kSpinLimit) {
-          if (lane == 0) atomicCAS(k.c.status, 0, int(nb::kTimeoutFull));
-          do {
-            for (uint32_t j = 0; j < nb::kSpinLimit; ++j)
-              if (nb::mbar_try_wait(&bars[warp][slot], parity)) break;
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
-            if (slot == 0) parity ^= 1;
-          } while (slot != feed_slot);
-          return false;
-        }
-    }
-    return true;
+    for (uint32_t i = 0; i < k.polls; ++i)
+      if (__all_sync(0xffffffffu, nb::mbar_try_wait(&bars[warp][slot], parity))) return true;
+    if (lane == 0) atomicCAS(k.c.status, 0, int(nb::kTimeoutFull));
+    do {
+      for (uint32_t j = 0; j < nb::kSpinLimit; ++j)
+        if (nb::mbar_try_wait(&bars[warp][slot], parity)) break;
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+      if (slot == 0) parity ^= 1;
+    } while (slot != feed_slot);
+    __syncwarp();
+    return false;
   };
   auto release = [&]() {
     __syncwarp();
@@ -745,7 +742,32 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     if (slot == 0) parity ^= 1;
   };
 
-  long pos = k.by_task ? long(blockIdx.x) : cuts.begin(unit), pos_end = k.by_task ? total : cuts.begin(unit + 1);
+  // (floats of a column's piece: its output, not yet divided, the maximum and the sum)
+  const int width = 8 * U + 2;
+  // by tasks: joins what the warps left in their rings; all warps call it together
+  auto join_task = [&](const ListWork& w, int h, int tile) {
+    __syncthreads();
+    const int n = min(COLS, w.n * k.a.group - tile * COLS);
+    for (int i = threadIdx.x; i < n * D; i += WARPS * 32) {
+      const int in_tile = i / D, d = i - in_tile * D, c = tile * COLS + in_tile, row = c / k.a.group;
+      const float* from = reinterpret_cast<const float*>(smem) + in_tile * width;
+      float top = -INFINITY, x = 0.f, z = 0.f;
+#pragma unroll
+      for (int q = 0; q < WARPS; ++q) top = fmaxf(top, from[q * (STAGES * stage / 4) + 8 * U]);
+#pragma unroll
+      for (int q = 0; q < WARPS; ++q) {
+        const float m = from[q * (STAGES * stage / 4) + 8 * U], f = m == top ? 1.f : ex2(m - top);
+        x += f * from[q * (STAGES * stage / 4) + d];
+        z += f * from[q * (STAGES * stage / 4) + 8 * U + 1];
+      }
+      reinterpret_cast<T*>(k.a.out)[long(w.s0 + row) * k.a.o_row + long(h * k.a.group + c - row * k.a.group) * k.a.o_head + d] =
+          from_f<T>(z == 0.f ? 0.f : x / z);
+    }
+    nb::fence_async_smem();      // (the rings are written by copies again)
+    __syncthreads();
+  };
+
+  long pos = k.by_task ? long(blockIdx.x) : cuts.begin(unit), pos_end = k.by_task ? total : cuts.begin(unit + 1), run_from = 0;
   while (true) {
     if (pos >= pos_end) {
       if (unit_next < 0) break;
@@ -757,7 +779,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     const Run run = run_at(k, cum, lists, pos, pos_end, COLS, warp, WARPS);
     const ListWork w = run.w;
     const int h = run.h, tile = run.tile, b0 = run.b, b1 = run.b + run.blocks;
-    const long run_from = pos;
+    run_from = pos;
     pos += k.by_task ? long(gridDim.x) : run.blocks;
     if (k.by_task) {
       feed_at = ((long(run.l) * k.c.H + run.h) * k.c.nb + run.b) * long(half);
@@ -857,7 +879,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
       }
       const float ks_now = __shfl_sync(0xffffffffu, ks_32, in_32), vs_now = __shfl_sync(0xffffffffu, vs_32, in_32);
       // ---- scores of 64 entries
-      if (!landed()) return;
+      if (!landed()) goto gave_up;
       const uint32_t keys_at = ring_at + slot * stage;
       float s[NT][4][4];
 #pragma unroll
@@ -956,7 +978,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
           }
       }
       // ---- output of these entries
-      if (HALVES == 1 && !landed()) return;
+      if (HALVES == 1 && !landed()) goto gave_up;
       const uint32_t values_at = ring_at + slot * stage + (HALVES - 1) * half;
       const bool past_end = CODE != 0 && (b + 1) * kBlock > w.len;
       // (the last pair first: its spare rows bring the sums of the weights, from which the others' bias follows)
@@ -1044,7 +1066,6 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
 
     // ---- the piece's result
     const bool whole = !k.by_task && b0 == 0 && b1 == w.nb;
-    const int width = 8 * U + 2;
     // (by tasks into the warp's own ring, which holds nothing by now)
     float* to_piece = k.by_task ? reinterpret_cast<float*>(ring) : k.ws + long(2 * unit + (b0 == 0 ? 1 : 0)) * COLS * width;
     int pieces = 1;
@@ -1080,27 +1101,45 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
         }
         if (!k.by_task && b0 == 0 && g == 0) k.cut[long(w.s0 + row) * k.c.H * k.a.group + head] = make_int2(unit, pieces * 16 + in_tile);
       }
-    if (k.by_task) {
-      __syncthreads();
-      const int n = min(COLS, w.n * k.a.group - tile * COLS);
-      for (int i = threadIdx.x; i < n * D; i += WARPS * 32) {
-        const int in_tile = i / D, d = i - in_tile * D, c = tile * COLS + in_tile, row = c / k.a.group;
-        const float* from = reinterpret_cast<const float*>(smem) + in_tile * width;
-        float top = -INFINITY, x = 0.f, z = 0.f;
-#pragma unroll
-        for (int q = 0; q < WARPS; ++q) top = fmaxf(top, from[q * (STAGES * stage / 4) + 8 * U]);
-#pragma unroll
-        for (int q = 0; q < WARPS; ++q) {
-          const float m = from[q * (STAGES * stage / 4) + 8 * U], f = m == top ? 1.f : ex2(m - top);
-          x += f * from[q * (STAGES * stage / 4) + d];
-          z += f * from[q * (STAGES * stage / 4) + 8 * U + 1];
-        }
-        reinterpret_cast<T*>(k.a.out)[long(w.s0 + row) * k.a.o_row + long(h * k.a.group + c - row * k.a.group) * k.a.o_head + d] =
-            from_f<T>(z == 0.f ? 0.f : x / z);
+    if (k.by_task) join_task(w, h, tile);
+  }
+  return;
+
+gave_up:      // The warp copies nothing more, but walks through the rest of its work, units that it can still fetch
+              // included, and leaves NaN: every piece that a join reads is written, and no row looks computed.
+  pos = run_from;
+  while (true) {
+    if (pos >= pos_end) {
+      if (unit_next < 0 && more) {
+        int u = 0;
+        if (lane == 0) u = cuts.workers + atomicAdd(k.next, 1);
+        u = __shfl_sync(0xffffffffu, u, 0);
+        more = u < cuts.units;
+        if (more) unit_next = u;
       }
-      nb::fence_async_smem();      // (the rings are written by copies again)
-      __syncthreads();
+      if (unit_next < 0) break;
+      unit = unit_next;
+      unit_next = -1;
+      pos = cuts.begin(unit);
+      pos_end = cuts.begin(unit + 1);
     }
+    const Run run = run_at(k, cum, lists, pos, pos_end, COLS, warp, WARPS);
+    const ListWork& w = run.w;
+    const bool whole = !k.by_task && run.b == 0 && run.blocks == w.nb;
+    const int n = min(COLS, w.n * k.a.group - run.tile * COLS), pieces = whole ? 1 : cuts.of(pos + w.nb - 1) - unit + 1;
+    const float nan = __uint_as_float(0x7fc00000u);
+    float* piece = k.by_task ? reinterpret_cast<float*>(ring) : k.ws + long(2 * unit + (run.b == 0 ? 1 : 0)) * COLS * width;
+    for (int i = lane; i < n * (whole ? D : width); i += 32) {
+      const int in_tile = i / D, c = run.tile * COLS + in_tile, row = c / k.a.group, head = run.h * k.a.group + c - row * k.a.group;
+      if (whole) reinterpret_cast<T*>(k.a.out)[long(w.s0 + row) * k.a.o_row + long(head) * k.a.o_head + i - in_tile * D] = from_f<T>(nan);
+      else piece[i] = nan;
+    }
+    if (!k.by_task && run.b == 0 && lane < n) {
+      const int c = run.tile * COLS + lane, row = c / k.a.group;
+      k.cut[long(w.s0 + row) * k.c.H * k.a.group + run.h * k.a.group + c - row * k.a.group] = make_int2(unit, pieces * 16 + lane);
+    }
+    pos += k.by_task ? long(gridDim.x) : run.blocks;
+    if (k.by_task) join_task(w, run.h, run.tile);
   }
 }
 
@@ -1347,7 +1386,8 @@ long nb_kv8_attention_workspace(int L, int H, int nb, int D, int rows, int max_r
   return nbk::plan_of(L, H, nb, D, rows, max_rows, group).bytes;
 }
 
-int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long ws_bytes, cudaStream_t st) {
+// `polls`: looks at a copy's barrier before a wait for it gives up (0: at once).
+int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long ws_bytes, unsigned polls, cudaStream_t st) {
   using namespace nbk;
   if (bad_cache(c) || a->rows < 0 || a->group < 1 || a->max_rows < 1) return -1;
   // (a list's tasks are counted in 32 bits)
@@ -1364,6 +1404,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
   k.c = *c;
   k.a = *a;
   k.by_task = plan.by_task;
+  k.polls = polls;
   k.dynamic = k.workers = 0;
   k.next = k.bad = nullptr;
   k.cut = nullptr;

@@ -49,7 +49,7 @@ def _L():
         L.nb_kv8_append.argtypes = [p(CacheArgs), p(RowArgs), vp]
         L.nb_kv8_truncate.argtypes = [p(CacheArgs), vp, vp]
         L.nb_kv8_read.argtypes = [p(CacheArgs), p(RowArgs), C.c_int, vp]
-        L.nb_kv8_attention.argtypes = [p(CacheArgs), p(AttentionArgs), vp, C.c_long, vp]
+        L.nb_kv8_attention.argtypes = [p(CacheArgs), p(AttentionArgs), vp, C.c_long, C.c_uint, vp]
         L.nb_kv8_attention_workspace.argtypes = [C.c_int] * 7
         L.nb_verify_draft.argtypes = [p(VerifyArgs), vp]
         for f in (L.nb_kv8_append, L.nb_kv8_truncate, L.nb_kv8_read, L.nb_kv8_attention, L.nb_verify_draft):
@@ -116,6 +116,7 @@ def kv8_read(cache: KV8Cache, seg_start: Tensor, start: Tensor, rows: int, dtype
 
 
 LOG2E = math.log2(math.e)
+WAIT_POLLS = 1 << 24       # looks at a copy of codes before the attention's wait for it gives up (status word, NaN rows)
 _sizes: dict = {}          # bytes of workspace for a shape (a function of the shape and the device alone)
 
 
@@ -145,7 +146,7 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     ws = lengths.new_empty(-(-size // 4)) if size else None
     a = AttentionArgs(q.data_ptr(), out.data_ptr(), q_row, q_head, o_row, o_head, seg_start.data_ptr(), lengths.data_ptr(), rows,
                       max_rows, group, FLOATS[q.dtype], 0 if given else 1, scale * LOG2E)
-    _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, None if ws is None else ws.data_ptr(), size,
+    _launch(L.nb_kv8_attention, cache.device, _cache_args(cache), a, None if ws is None else ws.data_ptr(), size, WAIT_POLLS,
             launches=1 if ws is None else 2)
     return out
 
