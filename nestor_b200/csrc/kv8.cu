@@ -257,7 +257,9 @@ __global__ void __launch_bounds__(256, NU == 1 ? 4 : 2) append_kernel(nb_kv8_cac
     const int s0 = p.seg[l], s1 = p.seg[l + 1], at = p.start[l];
     if (s0 > r || s1 <= r || s0 < 0) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
-      return;
+      if (s0 <= r) return;
+      r = s0;      // (rows before the first list)
+      continue;
     }
     if (s1 > end || at < 0 || long(at) + (s1 - s0) > cap) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
@@ -365,8 +367,10 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
     const int s0 = p.seg[l], s1 = p.seg[l + 1], at = p.start[l];
     if (s0 > r || s1 <= r || s0 < 0) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
-      zeros(r, r1);
-      return;
+      zeros(r, s0 > r ? min(s0, r1) : r1);
+      if (s0 <= r) return;
+      r = s0;
+      continue;
     }
     if (s1 > end || at < 0 || long(at) + (s1 - s0) > cap) {
       if (threadIdx.x == 0) atomicCAS(c.status, 0, kStatusRange);
@@ -445,6 +449,7 @@ struct Attn {
   int2* cut;          // [rows][query heads]: of the item's task the first unit; the number of pieces * 16 + the item's column
   float* ws;          // pieces: slot 2u for a task that unit u continues, 2u + 1 for one that it begins
   int workers, dynamic, by_task;
+  int first;          // whether these lists are the first (their rows begin at 0)
   unsigned polls;     // looks at a copy's barrier before the wait for it gives up
 };
 
@@ -629,6 +634,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
     lists[3 * l + 1] = w.n;
     lists[3 * l + 2] = w.len;
     bad = bad || k.a.seg[l + 1] > min(k.a.rows, seg_end) || k.a.seg[l] < 0 || k.a.seg[l + 1] < k.a.seg[l];
+    bad = bad || (k.first && l == 0 && w.s0 != 0);
     if (k.a.len[l] > k.c.nb * kBlock && blockIdx.x == 0) atomicCAS(k.c.status, 0, kStatusRange);
   }
   if (lane < STAGES) nb::mbar_init(&bars[warp][lane], 1);
@@ -660,7 +666,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   const long total = cum[L];
   if (k.by_task && (k.a.zero_tail || bad))      // (with units attn_join does this)
     for (int r = blockIdx.x * WARPS + warp; r < k.a.rows; r += gridDim.x * WARPS)
-      if (r >= seg_end ? k.a.zero_tail : r >= k.a.seg[0] && bad && !covered(k, r, seg_end, COLS))
+      if (r >= seg_end ? k.a.zero_tail : bad && !covered(k, r, seg_end, COLS))
         for (int i = lane; i < k.c.H * k.a.group * D; i += 32)
           reinterpret_cast<T*>(k.a.out)[long(r) * k.a.o_row + long(i / D) * k.a.o_head + i % D] = from_f<T>(0.f);
   if (total == 0) return;
@@ -1156,7 +1162,7 @@ __global__ void __launch_bounds__((TEAM < 4 ? 4 : TEAM) * 32) attn_join(const At
   const int row = int(item / heads), head = int(item - long(row) * heads);
   const int L = k.c.L, D = k.c.D, width = 8 * k.c.U + 2, seg_begin = k.a.seg[0], seg_end = k.a.seg[L];
   const bool exists = item < long(k.a.rows) * heads;
-  bool live = exists && row >= seg_begin && row < seg_end;
+  bool live = exists && (row >= seg_begin || k.first) && row < seg_end;      // (rows before the first list: bounds that are bad)
   const long at = long(row) * k.a.o_row + long(head) * k.a.o_head;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int2 cut = live ? k.cut[item] : make_int2(0, 0);
@@ -1404,6 +1410,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
   k.c = *c;
   k.a = *a;
   k.by_task = plan.by_task;
+  k.first = 1;
   k.polls = polls;
   k.dynamic = k.workers = 0;
   k.next = k.bad = nullptr;
@@ -1425,6 +1432,7 @@ int nb_kv8_attention(const nb_kv8_cache* c, const nb_kv8_attn* a, void* ws, long
       k.c.codes[i] = reinterpret_cast<uint8_t*>(c->codes[i]) + lh * c->U * 512;
       k.c.scale[i] = c->scale[i] + lh;
     }
+    k.first = l0 == 0;
     k.a.seg = a->seg + l0;
     k.a.len = a->len + l0;
     k.a.zero_tail = a->zero_tail && l0 + k.c.L >= c->L;

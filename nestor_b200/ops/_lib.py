@@ -102,7 +102,7 @@ def check_status(device: torch.device) -> None:
         status_word(device).zero_()
         why = "a bounded device-side wait gave up"
         if code == 7:
-            why = "rows beyond the capacity of a key/value list, or row bounds that do not ascend: those rows were dropped"
+            why = "rows beyond the capacity of a key/value list, or row bounds that do not ascend from 0: those rows were dropped"
         raise RuntimeError(f"nestor_b200 kernel reported status {code} ({why})")
 
 

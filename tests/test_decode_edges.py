@@ -1,9 +1,12 @@
 """The decoding ops and decode states at the edges: waits that run out, row bounds, threads, other callers' decode states."""
 
+import math
+
 import pytest
 import torch
 
 from nestor_b200 import ops
+from test_decode_ops import filled, same
 
 DEV = "cuda"
 
@@ -64,3 +67,46 @@ def test_a_wait_for_codes_that_runs_out_is_reported_and_leaves_nan(shape, code, 
     monkeypatch.undo()
     assert torch.equal(want, ops.kv8_attention(q, cache, seg, lengths, 0.05, max_rows=max(counts)))
     _lib.check_status(dev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("given", [False, True])
+@pytest.mark.parametrize("capacity", [64, 300_000])               # by tasks; by units with a workspace
+def test_rows_before_the_first_list_are_zeros_and_reported(capacity, given):
+    from nestor_b200.ops import _lib
+    dev = torch.device(DEV, 0)
+    cache, _, _ = filled([3, 50], 2, 24, torch.int8, torch.bfloat16, capacity=capacity, device=DEV)
+    q = torch.randn(7, 2, 24, device=DEV).bfloat16()
+    n = i32([3, 50], DEV)
+    want = ops.kv8_attention(q[2:], cache, seg_of([1, 2], DEV), n, 0.2, max_rows=2)
+    _lib.check_status(dev)
+    held = [torch.full_like(q, math.nan) for _ in range(8)]       # (what an allocation of this size finds)
+    out = torch.full_like(q, 3.0) if given else None
+    del held
+    got = ops.kv8_attention(q, cache, i32([2, 3, 5], DEV), n, 0.2, max_rows=2, out=out)
+    with pytest.raises(RuntimeError, match="row bounds"):
+        _lib.check_status(dev)
+    assert (got[:2] == 0).all() and torch.equal(got[2:5], want[:3]) and (got[5:] == (3 if given else 0)).all()
+
+
+@pytest.mark.gpu
+def test_rows_before_the_first_list_cost_no_other_row():
+    """Append drops them and read gives zeros for them, both report them, and the rows behind them are served."""
+
+    from nestor_b200.ops import _lib
+    dev = torch.device(DEV, 0)
+    a, b = (ops.kv8_cache(3, 2, 128, 24, DEV) for _ in range(2))
+    k, v = (torch.randn(9, 2, 24, device=DEV).bfloat16() for _ in range(2))
+    zero = i32([0, 0, 0], DEV)
+    ops.kv8_append(a, k[2:], v[2:], i32([0, 1, 1, 5], DEV), zero, max_rows=64)
+    want = ops.kv8_read(a, i32([0, 1, 1, 5], DEV), zero, 6, max_rows=64)
+    _lib.check_status(dev)
+    ops.kv8_append(b, k, v, i32([2, 3, 3, 7], DEV), zero, max_rows=64)
+    with pytest.raises(RuntimeError, match="row bounds"):
+        _lib.check_status(dev)
+    assert same(a, b)
+    got = ops.kv8_read(b, i32([2, 3, 3, 7], DEV), zero, 8, max_rows=64)
+    with pytest.raises(RuntimeError, match="row bounds"):
+        _lib.check_status(dev)
+    for x, y in zip(want, got):
+        assert (y[:2] == 0).all() and torch.equal(x, y[2:])
