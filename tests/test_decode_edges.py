@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from nestor_b200 import ops
-from test_decode_ops import filled, same
+from test_decode_ops import CODES, TYPES, filled, same, to, values64
 
 DEV = "cuda"
 
@@ -32,7 +32,7 @@ def random_cache(L, H, blocks, hd, code, seed, kind=torch.bfloat16):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("code", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("shape", [
     (6, 2, 8, 40, 1, [1, 1, 0, 1, 1, 1]),             # by tasks
     (5, 2, 8, 104, 2, [3, 1, 1, 0, 5]),               # by tasks, wide heads, two column tiles
@@ -110,3 +110,50 @@ def test_rows_before_the_first_list_cost_no_other_row():
         _lib.check_status(dev)
     for x, y in zip(want, got):
         assert (y[:2] == 0).all() and torch.equal(x, y[2:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("capacity", [1024, 20_032])              # the same entries by tasks and by units
+def test_small_weights_beside_a_dominating_one(code, kind, capacity):
+    """One entry 20 above all others, with the value zero: what is left are the others, each with e^-20 of its weight.
+
+    With ``m = sum_i p_i |v_i|``: scores and exponentials as in ``attention64``, whose relative error ``e`` of a weight
+    moves the output by at most ``2 e m`` here (all terms are kept, not bounded by the largest value); the weights, two
+    fp16 numbers, 2^-21 of themselves and 2^-40 of their block's largest one, which is theirs but for the first block; for
+    bf16, one number, 2^-11 of themselves and 2^-32 of the largest; the fp32 sums of products of one sign
+    ``(n / 16 + 16) 2^-23 m``. int8 codes with 16-bit queries enter as 128 more: the four to eight products of a block and the
+    removal of the 128 round sums of up to 128 times the block's weights, ``10 2^-23 128 sum(p)`` in all. The output is
+    rounded by half a step, which for outputs below the type's smallest normal number ``t`` (2^-14 in fp16; 1e-6 is below
+    it) is that of ``t``: ``t eps / 2`` = 2^-25.
+    """
+
+    n, hd = min(capacity, 20_001), 8
+    cache = ops.kv8_cache(1, 1, capacity, hd, DEV, code, torch.float32)
+    g = torch.Generator().manual_seed(4)
+    k = torch.zeros(n, 1, hd)
+    k[0, 0, 0] = 1
+    v = torch.rand(n, 1, hd, generator=g) * 0.5 + 0.5
+    v[0] = 0
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), seg_of([n], DEV), i32([0], DEV), max_rows=n)
+    q = torch.zeros(2, 1, hd)
+    q[0, 0, 0], q[1, 0, 0] = 20, 10
+    q = q.to(kind)
+    got = ops.kv8_attention(q.to(DEV), cache, seg_of([2], DEV), i32([n], DEV), 1.0, max_rows=2).double().cpu()
+    host = to(cache, "cpu")
+    for a in range(2):
+        see = n - 1 + a
+        kk, vv = (values64(host, w, 0, n)[0, :see] for w in ("k", "v"))
+        s = kk @ q[a, 0].double()
+        p = torch.softmax(s, 0)
+        want, m = p @ vv, p @ vv.abs()
+        lift = 128 if kind != torch.float32 and code == torch.int8 else 0
+        big = float(s.abs().max()) + lift * float(host.k_scale.max()) * float(q[a].abs().sum())
+        e = math.expm1(2 * (big * (hd + 8) * 2.0 ** -23 + 2.0 ** -22 + 2 * float(s.abs().max()) * 1.45 * 2.0 ** -23))
+        e += 2.0 ** -11 if kind == torch.bfloat16 else 2.0 ** -21
+        grain = n * 2.0 ** -32 if kind == torch.bfloat16 else 64 * 2.0 ** -40
+        sums = (see / 16 + 16) * 2.0 ** -23 * m + (10 * 2.0 ** -23 * 128 * float(host.v_scale.max()) if lift else 0.0)
+        tol = 2 * e * m + sums + grain + torch.finfo(kind).eps / 2 * (want.abs() * 1.01).clamp_min(torch.finfo(kind).tiny)
+        off = (got[a, 0] - want).abs()
+        assert (off <= tol).all(), (a, float((off / tol).max()), float((off / want).max()))
