@@ -423,8 +423,9 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // int8, 0.71 GB: 125 us, 5.7 TB/s with both launches). The tensor pipe is used because a column tile of 8 costs no more
 // than one query; the conversion (0.75 instructions a code) is then the largest part of a warp's work.
 //
-// Precision. q is scaled per column by a power of two, into [1, 2) or, where the products carry a factor 2^-24, into
-// [2^14, 2^15), and rounded to fp16 (exact for bf16 and fp16 queries, two fp16 numbers for fp32 ones). int8 codes x enter
+// Precision. q is scaled per column by a power of two that takes its largest element into [2^14, 2^15), and rounded to
+// fp16 (to two fp16 numbers for fp32 queries). fp16 elements above 2^-28 and bf16 elements above 2^-31 of the largest are
+// exact, fp32 elements above 2^-17 of it keep 22 bits, and no element is off by more than 2^-39 of it. int8 codes x enter
 // the products of 16-bit queries as 128 + x, so their fp32 sums carry 128 times the sum of the queries (of the weights),
 // which is taken off at the end: a rounding of such a sum is up to 2^-23 of that. The sum of the softmax adds the rounded weights.
 // For bf16 outputs (8 bits) a probability is one fp16 number, 2^7 at the running maximum: weights down to 2^-21 of the
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
   constexpr int PAIRS = (UMAX + 1) / 2, COLS = 8 * NT, STAGES = stages_of(UMAX), HALVES = halves_of(UMAX), WARPS = warps_of(UMAX, NT);
   // fp16 numbers that a query element and a probability are held in
   constexpr int QS = sizeof(T) == 4 ? 2 : 1, PS = std::is_same_v<T, __nv_bfloat16> ? 1 : 2;
-  // int8 codes enter the products as (128 + x) 2^-24, queries as [2^14, 2^15)
+  // int8 codes enter the products as (128 + x) 2^-24
   constexpr bool RAW = QS == 1, BIASED = RAW && CODE == 0;
   constexpr bool LOCAL = PS == 2;      // probabilities are relative to their own block's maximum
   constexpr float kUnit = BIASED ? 0x1p24f : 1.f;
@@ -840,8 +841,8 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      constexpr unsigned LIFT = BIASED ? 14 : 0;
-      const unsigned ex = min(max(__float_as_uint(top) >> 23, LIFT + 1u), 253u);       // biased exponent
+      constexpr unsigned LIFT = 14;
+      const unsigned ex = min(max(__float_as_uint(top) >> 23, LIFT + 1u), 254u);       // biased exponent
       const float down = __uint_as_float((254u + LIFT - ex) << 23), up = __uint_as_float((ex - LIFT) << 23);
       float q_sum = 0.f;
 #pragma unroll

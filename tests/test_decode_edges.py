@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from nestor_b200 import ops
-from test_decode_ops import CODES, TYPES, filled, same, to, values64
+from test_decode_ops import CODES, TYPES, check_attention, filled, same, to, values64
 
 DEV = "cuda"
 
@@ -157,3 +157,29 @@ def test_small_weights_beside_a_dominating_one(code, kind, capacity):
         tol = 2 * e * m + sums + grain + torch.finfo(kind).eps / 2 * (want.abs() * 1.01).clamp_min(torch.finfo(kind).tiny)
         off = (got[a, 0] - want).abs()
         assert (off <= tol).all(), (a, float((off / tol).max()), float((off / want).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("code", CODES)
+def test_queries_of_a_wide_range(code, kind):
+    """A large element where the keys are zero, and elements 2^-18 of it that decide against keys 2^12 times larger."""
+
+    n, hd = 90, 40
+    g = torch.Generator().manual_seed(6)
+    k = torch.randn(n, 1, hd, generator=g) * 2.0 ** 12
+    k[:, :, 3] = 0
+    v = torch.randn(n, 1, hd, generator=g)
+    cache = ops.kv8_cache(1, 1, 128, hd, DEV, code, torch.float32)
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), seg_of([n], DEV), i32([0], DEV), max_rows=n)
+    q = torch.randn(3, 1, hd, generator=g) * 2.0 ** -9
+    q[:, :, 3] = 2.0 ** 9 * 1.25
+    q = q.to(kind)
+    seg = seg_of([3], DEV)
+    got = ops.kv8_attention(q.to(DEV), cache, seg, i32([n], DEV), 0.25, max_rows=3)
+    host = to(cache, "cpu")
+    kk = values64(host, "k", 0, n)[0]
+    # (the bound without the zero keys' dimension: what stands there adds nothing to any score, but int8 codes carry it
+    # with a factor of 128, which is part of the bound)
+    assert float((kk @ q[0, 0].double()).abs().max()) > 8
+    check_attention(q, cache, seg, [n], 0.25, got)
