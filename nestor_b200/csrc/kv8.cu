@@ -862,7 +862,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
       // the score fragment holds columns 2t and 2t + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        qf[nt][i] = __shfl_sync(0xffffffffu, up, (2 * t + i) * 4) * k.a.scale_log2 * kUnit;
+        qf[nt][i] = __shfl_sync(0xffffffffu, up, (2 * t + i) * 4) * k.a.scale_log2;
         s_from[nt][i] = BIASED ? -128.f / kUnit * __shfl_sync(0xffffffffu, q_sum, (2 * t + i) * 4) : 0.f;
         const int c = tile * COLS + nt * 8 + 2 * t + i, row = c / k.a.group;
         see[nt][i] = row < w.n ? max(0, w.len - (w.n - 1 - row)) : 0;
@@ -870,6 +870,14 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
       }
     }
     seen_least = __reduce_min_sync(0xffffffffu, seen_least);
+    // Beyond 2^16 a fused product and difference, against a maximum that was rounded, can end above what fp16 holds. Where
+    // 32 blocks' scales allow such scores (a score is at most the factors times D codes times 2^15), both are rounded.
+    float q_top = qf[0][0];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) q_top = fmaxf(q_top, fmaxf(qf[nt][0], qf[nt][1]));
+    q_top = fmaxf(q_top, __shfl_xor_sync(0xffffffffu, q_top, 1));
+    q_top = fmaxf(q_top, __shfl_xor_sync(0xffffffffu, q_top, 2)) * (0.5f * (CODE == 0 ? 127.f : 448.f) * D);
+    bool far = __any_sync(0xffffffffu, q_top * ks_32 >= 1.f);
 
     // Sums of the weights come from the tensor pipe too: rows of ones, the unused second half of the last pair where
     // UMAX is odd, a product of their own where it is even.
@@ -892,7 +900,9 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
         ks_32 = ksp[b + lane];
         vs_32 = vsp[b + lane];
       }
-      const float ks_now = __shfl_sync(0xffffffffu, ks_32, in_32), vs_now = __shfl_sync(0xffffffffu, vs_32, in_32);
+      if (in_32 == 0 && b != b0) far = __any_sync(0xffffffffu, q_top * ks_32 >= 1.f);
+      // (kUnit here and not in qf, which it would take past fp32 for queries of 2^122 and more)
+      const float ks_now = __shfl_sync(0xffffffffu, ks_32, in_32) * kUnit, vs_now = __shfl_sync(0xffffffffu, vs_32, in_32);
       // ---- scores of 64 entries
       if (!landed()) goto gave_up;
       const uint32_t keys_at = ring_at + slot * stage;
@@ -920,7 +930,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
       if (HALVES == 1) release();
       // ---- softmax; a block in which some column's view ends takes the masked form
       const bool masked = (b + 1) * kBlock > seen_least;
-      float f[NT][2], vs_col[NT][2], off[NT][2], by_block[NT][2];      // by_block: factor on the block's sums (LOCAL)
+      float f[NT][2], vs_col[NT][2], base[NT][2], by_block[NT][2];      // by_block: factor on the block's sums (LOCAL)
       bool grows = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -950,7 +960,7 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * f[nt][i];
             const bool some = top > -INFINITY;      // (no entry of the block is visible, or all scores are NaN)
             const float now = fmaxf(mx[nt][i], top), keep = now == mx[nt][i] ? 1.f : ex2(mx[nt][i] - now);
-            off[nt][i] = some ? kTop - top : 0.f;
+            base[nt][i] = some ? top : 0.f;
             by_block[nt][i] = some ? ex2(top - now) : 0.f;
             vs_col[nt][i] *= by_block[nt][i];
             mx[nt][i] = now;
@@ -983,14 +993,32 @@ __global__ void __launch_bounds__(warps_of(UMAX, NT) * 32, 1) attn_kernel(const 
             }
           }
       }
+      if constexpr (!LOCAL)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) base[nt][i] = mx[nt][i];
+      if (far) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const float x = __fsub_rn(__fmul_rn(s[nt][m][2 * q + i], f[nt][i]), base[nt][i]);
+                s[nt][m][2 * q + i] = x > kSlack ? kSlack : x;      // (a NaN stays)
+              }
+            f[nt][i] = 1.f;
+            base[nt][i] = 0.f;
+          }
+      }
       unsigned pb[NT][4][2][PS];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        if constexpr (!LOCAL) {
-          off[nt][0] = kShift - mx[nt][0];
-          off[nt][1] = kShift - mx[nt][1];
-        }
-        const float2 from = make_float2(off[nt][0], off[nt][1]);
+        constexpr float SHIFT = LOCAL ? kTop : kShift;
+        const float2 from = make_float2(SHIFT - base[nt][0], SHIFT - base[nt][1]);
         const float2 by = make_float2(f[nt][0], f[nt][1]);
 #pragma unroll
         for (int m = 0; m < 4; ++m)

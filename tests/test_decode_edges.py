@@ -183,3 +183,25 @@ def test_queries_of_a_wide_range(code, kind):
     # with a factor of 128, which is part of the bound)
     assert float((kk @ q[0, 0].double()).abs().max()) > 8
     check_attention(q, cache, seg, [n], 0.25, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("top", [2.0 ** 100, 2.0 ** 124, 3.38e38])
+def test_queries_near_the_end_of_their_range(code, kind, top):
+    """Scores that differ by far more than the exponential can hold: the best entry's value (one weight, an exact sum),
+    rounded by half a step of the output's type."""
+
+    n, hd = 70, 8
+    g = torch.Generator().manual_seed(2)
+    k = torch.rand(n, 1, hd, generator=g) * 0.01
+    k[61, 0, 2] = 0.02
+    v = torch.randn(n, 1, hd, generator=g)
+    cache = ops.kv8_cache(1, 1, 128, hd, DEV, code, torch.float32)
+    ops.kv8_append(cache, k.to(DEV), v.to(DEV), seg_of([n], DEV), i32([0], DEV), max_rows=n)
+    q = torch.zeros(1, 1, hd)
+    q[0, 0, 2] = top
+    got = ops.kv8_attention(q.to(kind).to(DEV), cache, seg_of([1], DEV), i32([n], DEV), 1.0)[0, 0].double().cpu()
+    want = values64(to(cache, "cpu"), "v", 0, n)[0, 61]
+    assert ((got - want).abs() <= torch.finfo(kind).eps / 2 * want.abs() * 1.01 + 2.0 ** -20).all()
