@@ -10,6 +10,7 @@ machine the import fails loudly instead of silently running PyTorch ops.
 from __future__ import annotations
 
 import os
+import threading
 
 import torch
 
@@ -50,7 +51,16 @@ def oracle_path_report() -> dict[str, int]:
     return cuda_ops().oracle_path_report() if _cuda_mod is not None else {}
 
 
-_oracle_depth = 0
+_oracle_depth = 0                                  # oracle_ops regions of the process, whichever thread they are in
+_depth_lock = threading.Lock()
+
+
+class _Here(threading.local):
+    def __init__(self) -> None:
+        self.forced: list[bool] = []                # kernel_ops regions of this thread, and the oracle_ops regions in them
+
+
+_here = _Here()
 
 
 class oracle_ops:
@@ -63,37 +73,42 @@ class oracle_ops:
 
     def __enter__(self):
         global _oracle_depth
-        _oracle_depth += 1
+        with _depth_lock:
+            _oracle_depth += 1
+        if _here.forced:
+            _here.forced.append(False)
         return self
 
     def __exit__(self, *exc):
         global _oracle_depth
-        _oracle_depth -= 1
+        with _depth_lock:
+            _oracle_depth -= 1
+        if _here.forced:
+            _here.forced.pop()
         return False
 
 
 class kernel_ops:
     """``with ops.kernel_ops(on):`` run the ops of this block as kernels (``on`` false: as PyTorch statements) whatever
-    ``oracle_ops`` region it stands in. Stepwise decoding uses it: its per-token work runs as statements, its attention over
-    an 8-bit cache as the decode state was made."""
+    ``oracle_ops`` region it stands in. It holds for the calling thread alone. Stepwise decoding uses it: its per-token
+    work runs as statements, its attention over an 8-bit cache as the decode state was made."""
 
     def __init__(self, on: bool = True) -> None:
         self.on = on
 
     def __enter__(self):
-        global _oracle_depth
-        self.depth = _oracle_depth
-        _oracle_depth = 0 if self.on else 1
+        _here.forced.append(bool(self.on))
         return self
 
     def __exit__(self, *exc):
-        global _oracle_depth
-        _oracle_depth = self.depth
+        _here.forced.pop()
         return False
 
 
 def use_kernels(t: torch.Tensor) -> bool:
-    return t.is_cuda and not _FORCE_REF and _oracle_depth == 0
+    if not t.is_cuda or _FORCE_REF:
+        return False
+    return _here.forced[-1] if _here.forced else _oracle_depth == 0
 
 
 def _dispatch(name: str):

@@ -205,3 +205,73 @@ def test_queries_near_the_end_of_their_range(code, kind, top):
     got = ops.kv8_attention(q.to(kind).to(DEV), cache, seg_of([1], DEV), i32([n], DEV), 1.0)[0, 0].double().cpu()
     want = values64(to(cache, "cpu"), "v", 0, n)[0, 61]
     assert ((got - want).abs() <= torch.finfo(kind).eps / 2 * want.abs() * 1.01 + 2.0 ** -20).all()
+
+
+class OnDevice:
+    """What ``use_kernels`` looks at."""
+
+    is_cuda = True
+
+
+def test_regions_of_two_threads_do_not_mix():
+    """Two threads that decode at once enter and leave their regions in any order: each sees its own, and none is left."""
+
+    import threading
+    turn, seen, failed = [threading.Event() for _ in range(6)], {}, []
+
+    def wait(i):
+        if not turn[i].wait(20):
+            failed.append(i)
+
+    def a():
+        with ops.oracle_ops():
+            turn[0].set()
+            wait(1)                                               # b is in its region
+            with ops.kernel_ops(True):
+                turn[2].set()
+                seen["a"] = ops.use_kernels(OnDevice)
+                wait(3)                                           # b has left its region
+            seen["a behind"] = ops.use_kernels(OnDevice)
+        turn[4].set()
+
+    def b():
+        wait(0)
+        with ops.oracle_ops():
+            turn[1].set()
+            wait(2)                                               # a is in both
+            seen["b"] = ops.use_kernels(OnDevice)
+        turn[3].set()
+        wait(4)
+        seen["b behind"] = ops.use_kernels(OnDevice)
+
+    threads = [threading.Thread(target=f) for f in (a, b)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    assert seen == {"a": True, "a behind": False, "b": False, "b behind": True}
+    assert ops.use_kernels(OnDevice)
+
+
+def test_nested_regions():
+    at = lambda: ops.use_kernels(OnDevice)                        # noqa: E731
+    with ops.oracle_ops():
+        assert not at()
+        inner = ops.kernel_ops(True)
+        with inner:
+            assert at()
+            with ops.oracle_ops():
+                assert not at()
+                with inner:
+                    assert at()
+                assert not at()
+            assert at()
+        with ops.kernel_ops(False):
+            assert not at()
+        assert not at()
+    assert at()
+    with pytest.raises(KeyError):
+        with ops.oracle_ops(), ops.kernel_ops(True):
+            raise KeyError
+    assert at()
