@@ -9,6 +9,7 @@ machine the import fails loudly instead of silently running PyTorch ops.
 
 from __future__ import annotations
 
+import inspect
 import os
 import threading
 
@@ -136,9 +137,12 @@ def _dispatch_first(name: str):
     too often to look through all of them)."""
 
     ref_fn = getattr(_ref, name)
+    first = next(iter(inspect.signature(ref_fn).parameters))
 
     def op(*args, **kwargs):
-        if use_kernels(args[0] if args else next(iter(kwargs.values()))):
+        lead = args[0] if args else kwargs.get(first)
+        # (anything else, or nothing, is the statement's to refuse)
+        if isinstance(lead, (torch.Tensor, KV8Cache)) and use_kernels(lead):
             return getattr(cuda_ops(), name)(*args, **kwargs)
         return ref_fn(*args, **kwargs)
 

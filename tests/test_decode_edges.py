@@ -275,3 +275,27 @@ def test_nested_regions():
         with ops.oracle_ops(), ops.kernel_ops(True):
             raise KeyError
     assert at()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_keywords_in_any_order(device):
+    cache = ops.kv8_cache(2, 2, 64, 8, device)
+    rows = torch.randn(2, 2, 8, device=device).bfloat16()
+    seg, zero, one = (i32(x, device) for x in ([0, 1, 2], [0, 0], [1, 1]))
+    ops.kv8_append(max_rows=1, start=zero, seg_start=seg, v=rows, k=rows, cache=cache)
+    ops.kv8_truncate(lengths=one, cache=cache)
+    back = ops.kv8_read(rows=2, start=zero, seg_start=seg, cache=cache)[1]
+    got = ops.kv8_attention(scale=0.5, max_rows=1, lengths=one, seg_start=seg, cache=cache, q=rows)
+    assert torch.equal(got, ops.kv8_attention(rows, cache, seg, one, 0.5))
+    assert torch.allclose(got.float(), back, rtol=2.0 ** -8)      # one entry: its value
+    p = torch.softmax(torch.randn(2, 3, 9, device=device), -1)
+    x, u, w = torch.zeros(2, 2, dtype=torch.int32, device=device), torch.rand(2, 2, device=device), torch.rand(2, device=device)
+    a = ops.verify_draft(draft_probs=None, sample_u=w, accept_u=u, draft_tokens=x, target_probs=p)
+    assert all(torch.equal(i, j) for i, j in zip(a, ops.verify_draft(p, x, None, u, w)))
+
+
+def test_calls_without_their_first_argument():
+    cache = ops.kv8_cache(1, 1, 64, 8)
+    for call in (lambda: ops.kv8_truncate(), lambda: ops.kv8_truncate(lengths=i32([1])), lambda: ops.kv8_attention(cache=cache, scale=1.0)):
+        with pytest.raises(TypeError, match="argument"):
+            call()
