@@ -20,6 +20,7 @@ import math
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 BLOCK = 64                                                     # entries of a block
 MAX_HEAD_DIM = 128
@@ -115,6 +116,10 @@ def check_no_grad(op: str, *tensors: Tensor | None) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{op} is a decoding op without a backward pass: call it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{op} is a decoding op without derivatives: it takes no dual tensors")
 
 
 def check_count(op: str, rows: int, max_rows: int) -> None:

@@ -299,3 +299,26 @@ def test_calls_without_their_first_argument():
     for call in (lambda: ops.kv8_truncate(), lambda: ops.kv8_truncate(lengths=i32([1])), lambda: ops.kv8_attention(cache=cache, scale=1.0)):
         with pytest.raises(TypeError, match="argument"):
             call()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_dual_tensors_are_refused(device):
+    """Forward-mode derivatives would be lost without a word, under no_grad too."""
+
+    import torch.autograd.forward_ad as fwd
+    cache = ops.kv8_cache(1, 1, 64, 8, device, open_dtype=torch.float32)
+    rows, seg, n = torch.randn(1, 1, 8, device=device), i32([0, 1], device), i32([0], device)
+    p = torch.full((1, 2, 4), 0.25, device=device)
+    x, u, w = torch.zeros(1, 1, dtype=torch.int32, device=device), torch.rand(1, 1, device=device), torch.rand(1, device=device)
+    with torch.no_grad(), fwd.dual_level():
+        dual, dual_p = fwd.make_dual(rows, rows), fwd.make_dual(p, p)
+        for call in (lambda: ops.kv8_append(cache, dual, rows, seg, n), lambda: ops.kv8_append(cache, rows, dual, seg, n),
+                     lambda: ops.kv8_attention(dual, cache, seg, n, 1.0), lambda: ops.kv8_attention(rows, cache, seg, n, 1.0, out=dual),
+                     lambda: ops.verify_draft(dual_p, x, None, u, w), lambda: ops.verify_draft(p, x, dual_p[:, :1], u, w)):
+            with pytest.raises(RuntimeError, match="dual tensors"):
+                call()
+        ops.kv8_append(cache, rows, rows, seg, n)                # (others are welcome inside such a level)
+        ops.kv8_attention(rows, cache, seg, n + 1, 1.0)
+        ops.verify_draft(p, x, p[:, :1], u, w)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda q: ops.kv8_attention(q, cache, seg, n + 1, 1.0), (rows,), (rows,))
