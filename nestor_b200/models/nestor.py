@@ -427,6 +427,9 @@ class LayerKV8Cache:
             ops.kv8_truncate(self.kv, self.count)
 
 
+EIGHT_BIT = (torch.int8, torch.float8_e4m3fn)      # dtypes of an 8-bit decode state
+
+
 class NestorKVCache:
     """Decode state of the whole backbone: one ``LayerKVCache`` (``LayerKV8Cache`` for ``dtype`` int8 or float8_e4m3fn)
     per (block, layer).
@@ -438,7 +441,7 @@ class NestorKVCache:
     TAKE_BACK = 64
 
     def __init__(self, backbone: "Nestor", B: int, max_len: int, device, dtype=torch.float32, open_dtype=torch.float32) -> None:
-        self.eight_bit = dtype in (torch.int8, torch.float8_e4m3fn)
+        self.eight_bit = dtype in EIGHT_BIT
 
         def layer(s):
             if self.eight_bit:

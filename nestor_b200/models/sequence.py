@@ -20,7 +20,7 @@ from nestor_b200.configs.model import (
     LanguageModelingHeadConfig, NestorConfig, ReferenceMupConfig, SequenceModelConfig, TextAdapterConfig,
 )
 from nestor_b200.models.modules import LayerStack, Matrix
-from nestor_b200.models.nestor import Nestor, NestorKVCache, W
+from nestor_b200.models.nestor import EIGHT_BIT, Nestor, NestorKVCache, W
 from nestor_b200.models.registry import (
     ADAPTERS, BACKBONES, HEADS, MODELS, register_adapter, register_backbone, register_head, register_model,
 )
@@ -320,6 +320,8 @@ class SequenceModel(nn.Module):
         lets a step feed several tokens at once."""
 
         device = self.head.weight.device if device is None else device
+        if dtype not in EIGHT_BIT:      # (all that a backbone's own decode state has to take)
+            return self.backbone.init_kv_cache(batch_size, max_len, device, dtype)
         return self.backbone.init_kv_cache(batch_size, max_len, device, dtype, open_dtype=self._step_dtype(torch.device(device)))
 
     def _step_dtype(self, device: torch.device) -> torch.dtype:
@@ -329,14 +331,16 @@ class SequenceModel(nn.Module):
     def decode_step(self, ids: Tensor, cache, pos: Tensor | None = None) -> Tensor:
         """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` or ``[B, 1]`` (``cache`` is advanced).
         Several tokens ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n``
-        single steps otherwise."""
+        single steps otherwise. The decode state of a backbone other than ``Nestor`` needs no more than a ``length``, the
+        tokens fed so far."""
 
-        if ids.shape[0] != cache.batch:
-            raise ValueError(f"the cache decodes {cache.batch} sequences, got tokens for {ids.shape[0]}")
+        eight_bit, batch = getattr(cache, "eight_bit", False), getattr(cache, "batch", ids.shape[0])
+        if ids.shape[0] != batch:
+            raise ValueError(f"the cache decodes {batch} sequences, got tokens for {ids.shape[0]}")
         if ids.dim() == 2 and ids.shape[1] == 1:
             ids, pos = ids[:, 0], None if pos is None else pos.reshape(-1)
         if ids.dim() == 2:
-            if not cache.eight_bit:
+            if not eight_bit:
                 steps = [self.decode_step(ids[:, t], cache, None if pos is None else pos[:, t]) for t in range(ids.shape[1])]
                 return torch.stack(steps, dim=1) if steps else ids.new_zeros(*ids.shape, self.head.vocab_size, dtype=torch.float32)
             if ids.shape[1] == 0:
@@ -344,7 +348,9 @@ class SequenceModel(nn.Module):
         B = ids.shape[0]
         rows = ids.reshape(B, -1)
         if pos is None:
-            pos = cache.positions.unsqueeze(1) + torch.arange(rows.shape[1], device=ids.device)
+            at = getattr(cache, "positions", None)
+            at = torch.full((B,), cache.length, dtype=torch.long, device=ids.device) if at is None else at
+            pos = at.unsqueeze(1) + torch.arange(rows.shape[1], device=ids.device)
             pos = pos if ids.dim() == 2 else pos.squeeze(1)
         cd = self._step_dtype(ids.device)
         x0 = self.adapter(rows).reshape(rows.numel(), -1)
@@ -355,7 +361,7 @@ class SequenceModel(nn.Module):
         """Feed ``prompt [B, S]`` and return the logits after its last token (``None`` for an empty prompt): pieces of up to
         ``PREFILL`` tokens into an 8-bit cache, token by token otherwise."""
 
-        step = self.PREFILL if cache.eight_bit else 1
+        step = self.PREFILL if getattr(cache, "eight_bit", False) else 1
         logits = None
         for a in range(0, prompt.shape[1], step):
             logits = self.decode_step(prompt[:, a : a + step] if step > 1 else prompt[:, a], cache)
@@ -408,6 +414,9 @@ class SequenceModel(nn.Module):
         draft.eval()
         room = S0 + max_new_tokens + 2 * (n + 1)      # (a sequence may overshoot by a round and then waits, feeding rounds)
         caches = [m.init_kv_cache(B, room, dev, cache_dtype) for m in (self, draft)]
+        for m, cache in zip((self, draft), caches):
+            if not hasattr(cache, "rollback"):
+                raise ValueError(f"decoding with drafts takes tokens back, which the decode state of {type(m.backbone).__name__} does not offer")
         for m, cache in zip((self, draft), caches):
             m._prefill(prompt[:, :-1], cache)
         out = torch.zeros(B, room, dtype=prompt.dtype, device=dev)

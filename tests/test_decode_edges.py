@@ -322,3 +322,43 @@ def test_dual_tensors_are_refused(device):
         ops.verify_draft(p, x, p[:, :1], u, w)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda q: ops.kv8_attention(q, cache, seg, n + 1, 1.0), (rows,), (rows,))
+
+
+class SumState:
+    """A decode state of another backbone, with the one attribute that stepwise decoding has always asked for."""
+
+    def __init__(self, B, width, device):
+        self.length, self.sum = 0, torch.zeros(B, width, device=device)
+
+
+class SumBackbone(torch.nn.Module):
+    def init_kv_cache(self, batch_size, max_len, device, dtype=torch.float32):
+        assert dtype == torch.float32
+        return SumState(batch_size, 128, device)
+
+    def forward_step(self, x0, pos, cache, cd):
+        assert pos.tolist() == [cache.length] * x0.shape[0] and pos.dtype == torch.long
+        cache.sum = 0.7 * cache.sum + x0 * (1 + pos[0])
+        cache.length += 1
+        return cache.sum.to(cd), {}
+
+
+def test_another_backbones_decode_state(tiny_scale):
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "dense", 2)
+    m.backbone = SumBackbone()
+    ids = torch.randint(0, 100263, (2, 6))
+    x = m.adapter(ids)
+    with torch.no_grad():
+        state, want = torch.zeros(2, x.shape[-1]), []
+        for t in range(6):
+            state = 0.7 * state + x[:, t] * (1 + t)
+            want.append(m.head(state, torch.float32).float())
+    cache = m.init_kv_cache(2, 6)
+    for t in range(3):
+        assert torch.equal(m.decode_step(ids[:, t], cache), want[t])
+    assert torch.equal(m.decode_step(ids[:, 3:], cache), torch.stack(want[3:], 1))       # several tokens: step by step
+    out = m.generate(ids, 4)
+    assert out.shape == (2, 10) and torch.equal(out[:, :6], ids) and torch.equal(out[:, 6], want[5].argmax(-1))
+    with pytest.raises(ValueError, match="SumBackbone does not offer"):
+        m.generate(ids, 4, draft=m)
