@@ -457,8 +457,10 @@ class NestorKVCache:
         self.recent: list[Tensor | None] = [None] * len(self.blocks)
 
     def note(self, block: int, idx: Tensor) -> None:
-        """Remember the columns ``idx [B, S, k]`` of a step's tokens in ``block``."""
+        """Remember the columns ``idx [B, S, k]`` of a step's tokens in ``block`` (fewer sequences: none of the others')."""
 
+        if idx.shape[0] < self.batch:
+            idx = torch.cat((idx, idx.new_full((self.batch - idx.shape[0], *idx.shape[1:]), -1)))
         old = self.recent[block]
         self.recent[block] = (idx if old is None else torch.cat((old, idx), dim=1))[:, -self.TAKE_BACK :]
 
@@ -997,10 +999,10 @@ class Nestor(Backbone):
             raise RuntimeError("forward_step is an evaluation path: call model.eval() first")
         if not self.config.causal:
             raise RuntimeError("stepwise decoding needs a causal model: a bidirectional token sees later ones")
-        B = cache.batch
-        S = x0.shape[0] // B
+        B = cache.batch if cache.eight_bit else min(cache.batch, x0.shape[0])
+        S = x0.shape[0] // B if B else 0
         if x0.shape[0] != B * S or S < 1 or (S > 1 and not cache.eight_bit):
-            raise ValueError(f"a step feeds one token to each of the cache's {B} sequences"
+            raise ValueError(f"a step feeds one token to each of the cache's {cache.batch} sequences"
                              f"{', or the same number to each' if cache.eight_bit else ''}; got {x0.shape[0]} rows")
         if cache.eight_bit and cache.length + S > cache.max_len:
             raise ValueError(f"key/value cache of {cache.max_len} positions per column is full")

@@ -331,11 +331,11 @@ class SequenceModel(nn.Module):
     def decode_step(self, ids: Tensor, cache, pos: Tensor | None = None) -> Tensor:
         """Logits ``[B, V]`` of the next position given the new tokens ``ids [B]`` or ``[B, 1]`` (``cache`` is advanced).
         Several tokens ``ids [B, n]`` give ``[B, n, V]``, the logits after each of them: one pass over an 8-bit cache, ``n``
-        single steps otherwise. The decode state of a backbone other than ``Nestor`` needs no more than a ``length``, the
-        tokens fed so far."""
+        single steps otherwise. An fp32 state may be stepped with fewer sequences than it holds, the first of them. The
+        decode state of a backbone other than ``Nestor`` needs no more than a ``length``, the tokens fed so far."""
 
         eight_bit, batch = getattr(cache, "eight_bit", False), getattr(cache, "batch", ids.shape[0])
-        if ids.shape[0] != batch:
+        if ids.shape[0] > batch or (eight_bit and ids.shape[0] != batch):
             raise ValueError(f"the cache decodes {batch} sequences, got tokens for {ids.shape[0]}")
         if ids.dim() == 2 and ids.shape[1] == 1:
             ids, pos = ids[:, 0], None if pos is None else pos.reshape(-1)
@@ -349,7 +349,7 @@ class SequenceModel(nn.Module):
         rows = ids.reshape(B, -1)
         if pos is None:
             at = getattr(cache, "positions", None)
-            at = torch.full((B,), cache.length, dtype=torch.long, device=ids.device) if at is None else at
+            at = torch.full((B,), cache.length, dtype=torch.long, device=ids.device) if at is None else at[:B]
             pos = at.unsqueeze(1) + torch.arange(rows.shape[1], device=ids.device)
             pos = pos if ids.dim() == 2 else pos.squeeze(1)
         cd = self._step_dtype(ids.device)

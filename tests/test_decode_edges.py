@@ -362,3 +362,37 @@ def test_another_backbones_decode_state(tiny_scale):
     assert out.shape == (2, 10) and torch.equal(out[:, :6], ids) and torch.equal(out[:, 6], want[5].argmax(-1))
     with pytest.raises(ValueError, match="SumBackbone does not offer"):
         m.generate(ids, 4, draft=m)
+
+
+def test_an_fp32_state_steps_its_first_sequences(tiny_scale):
+    """A state made for four sequences decodes two of them, then all: positions count steps, as they always did, and
+    taking tokens back touches the sequences that were fed."""
+
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "nestor", 4)
+    ids = torch.randint(0, 100263, (4, 9))
+    two, four = m.init_kv_cache(2, 12), m.init_kv_cache(4, 12)
+    for t in range(4):
+        assert torch.equal(m.decode_step(ids[:2, t], two), m.decode_step(ids[:2, t], four))
+    assert four.length == 4 and four.positions.tolist() == [4] * 4
+    alone = m.init_kv_cache(4, 12)
+    for t in range(4):
+        m.decode_step(ids[:, t], alone)
+    for blk in alone.blocks:
+        for layer in blk:
+            layer.count[2:] = 0                                   # (what the two that were not fed hold: nothing)
+    assert torch.allclose(m.decode_step(ids[:, 4], four), m.decode_step(ids[:, 4], alone), atol=1e-5)
+    four.rollback(torch.tensor([2, 1, 1, 0]))                     # (one step is all that the last two can give back)
+    assert four.positions.tolist() == [3, 4, 4, 5]
+    four.rollback(torch.tensor([0, 0, 0, 1]))
+    with pytest.raises(ValueError, match="taken back"):
+        four.rollback(torch.tensor([0, 0, 0, 1]))
+    with torch.no_grad():
+        full = m(ids[:2]).pred.float()
+    step = m.decode_step(torch.stack([ids[0, 3], ids[1, 4], ids[2, 4], ids[3, 4]]), four)
+    assert torch.allclose(step[0], full[0, 3], atol=2e-4, rtol=1e-4) and torch.allclose(step[1], full[1, 4], atol=2e-4, rtol=1e-4)
+    for state in (two, m.init_kv_cache(2, 8, dtype=torch.int8)):
+        with pytest.raises(ValueError, match="tokens for 3"):
+            m.decode_step(ids[:3, 0], state)
+    with pytest.raises(ValueError, match="tokens for 1"):
+        m.decode_step(ids[:1, 0], m.init_kv_cache(2, 8, dtype=torch.int8))
