@@ -451,10 +451,23 @@ class NestorKVCache:
         self.blocks = [[layer(blk.spec) for _ in blk.layers] for blk in backbone.blocks]
         self.columns = [blk.spec.G for blk in backbone.blocks]
         self.batch, self.max_len = B, max_len
-        self.length = 0
+        self._length = 0
         self.positions = torch.zeros(B, dtype=torch.long, device=device)
         # per block, the columns [B, <= TAKE_BACK, k] of every sequence's newest tokens, oldest first (-1: none)
         self.recent: list[Tensor | None] = [None] * len(self.blocks)
+
+    @property
+    def length(self) -> int:
+        """The largest position. Setting it (a state whose counts a program resets, to use it again) sets every sequence's
+        position; what was fed before cannot be taken back then."""
+
+        return self._length
+
+    @length.setter
+    def length(self, value: int) -> None:
+        self._length = value
+        self.positions = torch.full_like(self.positions, value)
+        self.recent = [None] * len(self.blocks)
 
     def note(self, block: int, idx: Tensor) -> None:
         """Remember the columns ``idx [B, S, k]`` of a step's tokens in ``block`` (fewer sequences: none of the others')."""
@@ -466,7 +479,7 @@ class NestorKVCache:
 
     def advance(self, tokens: int) -> None:
         self.positions = self.positions + tokens
-        self.length += tokens
+        self._length += tokens
 
     def rollback(self, dropped: Tensor) -> None:
         """Take back the newest ``dropped [B]`` tokens of every sequence (at most ``TAKE_BACK`` since they were fed)."""
@@ -491,7 +504,7 @@ class NestorKVCache:
             for cache in layers:
                 cache.take_back(drop)
         self.positions = self.positions - dropped
-        self.length = int(self.positions.max())
+        self._length = int(self.positions.max())
 
 
 class BlockContext:

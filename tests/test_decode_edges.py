@@ -396,3 +396,21 @@ def test_an_fp32_state_steps_its_first_sequences(tiny_scale):
             m.decode_step(ids[:3, 0], state)
     with pytest.raises(ValueError, match="tokens for 1"):
         m.decode_step(ids[:1, 0], m.init_kv_cache(2, 8, dtype=torch.int8))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int8])
+def test_a_decode_state_is_reset_by_its_counts_and_length(dtype, tiny_scale):
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "nestor", 5)
+    ids = torch.randint(0, 100263, (2, 5))
+    cache = m.init_kv_cache(2, 6, dtype=dtype)
+    first = [m.decode_step(ids[:, t], cache) for t in range(5)]
+    for blk in cache.blocks:
+        for layer in blk:
+            layer.count.zero_()
+    cache.length = 0
+    assert cache.positions.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="taken back"):
+        cache.rollback(torch.tensor([1, 1]))
+    assert all(torch.equal(first[t], m.decode_step(ids[:, t], cache)) for t in range(5))
+    assert cache.length == 5
