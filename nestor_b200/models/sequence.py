@@ -345,6 +345,12 @@ class SequenceModel(nn.Module):
                 return torch.stack(steps, dim=1) if steps else ids.new_zeros(*ids.shape, self.head.vocab_size, dtype=torch.float32)
             if ids.shape[1] == 0:
                 return ids.new_zeros(*ids.shape, self.head.vocab_size, dtype=torch.float32)
+        cd = self._step_dtype(ids.device)
+        return self.head(self._step(ids, cache, pos, cd), cd).float().view(*ids.shape, -1)
+
+    def _step(self, ids: Tensor, cache, pos: Tensor | None, cd: torch.dtype) -> Tensor:
+        """The head's input for the new tokens ``ids [B]`` or ``[B, n]``, a row for each (``cache`` is advanced)."""
+
         B = ids.shape[0]
         rows = ids.reshape(B, -1)
         if pos is None:
@@ -352,20 +358,26 @@ class SequenceModel(nn.Module):
             at = torch.full((B,), cache.length, dtype=torch.long, device=ids.device) if at is None else at[:B]
             pos = at.unsqueeze(1) + torch.arange(rows.shape[1], device=ids.device)
             pos = pos if ids.dim() == 2 else pos.squeeze(1)
-        cd = self._step_dtype(ids.device)
         x0 = self.adapter(rows).reshape(rows.numel(), -1)
         h, _ = self.backbone.forward_step(x0, pos, cache, cd)
-        return self.head(h, cd).float().view(*ids.shape, -1)
+        return h
 
     def _prefill(self, prompt: Tensor, cache) -> Tensor | None:
         """Feed ``prompt [B, S]`` and return the logits after its last token (``None`` for an empty prompt): pieces of up to
-        ``PREFILL`` tokens into an 8-bit cache, token by token otherwise."""
+        ``PREFILL`` tokens into an 8-bit cache, token by token otherwise. (A piece asks the head for its last row alone: the
+        logits of 512 tokens of 64 sequences would take 13 GB.)"""
 
-        step = self.PREFILL if getattr(cache, "eight_bit", False) else 1
-        logits = None
-        for a in range(0, prompt.shape[1], step):
-            logits = self.decode_step(prompt[:, a : a + step] if step > 1 else prompt[:, a], cache)
-        return logits if logits is None or logits.dim() == 2 else logits[:, -1]
+        B, S = prompt.shape
+        if S == 0:
+            return None
+        if not getattr(cache, "eight_bit", False):
+            for t in range(S):
+                logits = self.decode_step(prompt[:, t], cache)
+            return logits
+        cd = self._step_dtype(prompt.device)
+        for a in range(0, S, self.PREFILL):
+            h = self._step(prompt[:, a : a + self.PREFILL], cache, None, cd)
+        return self.head(h.view(B, -1, h.shape[-1])[:, -1].contiguous(), cd).float()
 
     PREFILL = 512
 

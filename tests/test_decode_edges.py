@@ -414,3 +414,22 @@ def test_a_decode_state_is_reset_by_its_counts_and_length(dtype, tiny_scale):
         cache.rollback(torch.tensor([1, 1]))
     assert all(torch.equal(first[t], m.decode_step(ids[:, t], cache)) for t in range(5))
     assert cache.length == 5
+
+
+@pytest.mark.parametrize("S", [37, 33, 16, 1])
+def test_a_prompt_asks_the_head_for_its_last_row(S, tiny_scale, monkeypatch):
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "nestor", 6)
+    monkeypatch.setattr(m, "PREFILL", 16)
+    prompt = torch.randint(0, 100263, (2, S))
+    asked, head = [], m.head.forward
+    monkeypatch.setattr(m.head, "forward", lambda h, *a, **kw: (asked.append(h.shape[0]), head(h, *a, **kw))[1])
+    with torch.no_grad():
+        got = m._prefill(prompt, m.init_kv_cache(2, 40, dtype=torch.int8))
+    assert asked == [2] and m._prefill(prompt[:, :0], m.init_kv_cache(2, 4, dtype=torch.int8)) is None
+    cache = m.init_kv_cache(2, 40, dtype=torch.int8)
+    for a in range(0, S, 16):
+        want = m.decode_step(prompt[:, a : a + 16], cache)
+    assert torch.allclose(got, want if want.dim() == 2 else want[:, -1], atol=1e-5)
+    out = m.generate(prompt, 2, cache_dtype=torch.int8)
+    assert torch.equal(out[:, S], got.argmax(-1))
