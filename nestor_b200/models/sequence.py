@@ -8,6 +8,7 @@ contract: pre-tokenised tensors carry no attention mask), ``nestor/heads/languag
 
 from __future__ import annotations
 
+import contextlib
 import dataclasses as dc
 import os
 from typing import Any
@@ -217,6 +218,20 @@ def apply_recipe_variants(model: nn.Module, mup: ReferenceMupConfig) -> None:
 
 
 @register_model(SequenceModelConfig)
+@contextlib.contextmanager
+def _evaluating(*models: nn.Module):
+    """The models in evaluation mode, and as they were behind it, however it is left."""
+
+    was = [m.training for m in models]
+    for m in models:
+        m.eval()
+    try:
+        yield
+    finally:
+        for m, training in zip(models, was):
+            m.train(training)
+
+
 class SequenceModel(nn.Module):
     """adapter -> backbone -> head, each built from its config through the registries.
 
@@ -394,9 +409,13 @@ class SequenceModel(nn.Module):
         """
 
         if draft is not None:
-            return self._generate_with_draft(prompt, max_new_tokens, temperature, generator, cache_dtype, draft, draft_tokens)
-        was_training = self.training
-        self.eval()
+            with _evaluating(self, draft):
+                return self._generate_with_draft(prompt, max_new_tokens, temperature, generator, cache_dtype, draft, draft_tokens)
+        with _evaluating(self):
+            return self._generate(prompt, max_new_tokens, temperature, generator, cache_dtype)
+
+    def _generate(self, prompt: Tensor, max_new_tokens: int, temperature: float, generator: torch.Generator | None,
+                  cache_dtype: torch.dtype) -> Tensor:
         B, S0 = prompt.shape
         cache = self.init_kv_cache(B, S0 + max_new_tokens, prompt.device, cache_dtype)
         logits = self._prefill(prompt, cache)
@@ -408,7 +427,6 @@ class SequenceModel(nn.Module):
                 nxt = logits.argmax(dim=-1)
             out.append(nxt.unsqueeze(1))
             logits = self.decode_step(nxt, cache)
-        self.train(was_training)
         return torch.cat(out, dim=1)
 
     def _generate_with_draft(self, prompt: Tensor, max_new_tokens: int, temperature: float, generator: torch.Generator | None,
@@ -421,9 +439,7 @@ class SequenceModel(nn.Module):
             raise ValueError(f"draft_tokens must be in 1..{most - 1} (a refused round has to be taken back), got {n}")
         if S0 < 1:
             raise ValueError("decoding with drafts needs a prompt of at least one token")
-        dev, was = prompt.device, (self.training, draft.training)
-        self.eval()
-        draft.eval()
+        dev = prompt.device
         room = S0 + max_new_tokens + 2 * (n + 1)      # (a sequence may overshoot by a round and then waits, feeding rounds)
         caches = [m.init_kv_cache(B, room, dev, cache_dtype) for m in (self, draft)]
         for m, cache in zip((self, draft), caches):
@@ -470,8 +486,6 @@ class SequenceModel(nn.Module):
             end, last = end + kept, torch.where(live, token, last)
             for cache in caches:
                 cache.rollback(n + 1 - kept)
-        self.train(was[0])
-        draft.train(was[1])
         return out[:, : S0 + max_new_tokens]
 
     def fsdp2_wrap_order(self) -> list[nn.Module]:

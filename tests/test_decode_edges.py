@@ -433,3 +433,23 @@ def test_a_prompt_asks_the_head_for_its_last_row(S, tiny_scale, monkeypatch):
     assert torch.allclose(got, want if want.dim() == 2 else want[:, -1], atol=1e-5)
     out = m.generate(prompt, 2, cache_dtype=torch.int8)
     assert torch.equal(out[:, S], got.argmax(-1))
+
+
+def test_a_refused_or_failing_generation_leaves_the_training_mode(tiny_scale, monkeypatch):
+    from test_decode_8bit import tiny
+    m, draft = tiny(tiny_scale, "moe", 5).train(), tiny(tiny_scale, "dense", 6).train()
+    prompt = torch.randint(0, 100263, (2, 4))
+    with pytest.raises(ValueError, match="draft_tokens"):
+        m.generate(prompt, 4, draft=draft, draft_tokens=0)
+    with torch.no_grad():
+        m.head.weight.fill_(float("nan"))
+    with pytest.raises(RuntimeError, match="no token to draw"):
+        m.generate(prompt, 4, 0.8, torch.Generator().manual_seed(0), torch.int8, draft, 3)
+    assert m.training and draft.training and all(x.training for x in m.modules()) and all(x.training for x in draft.modules())
+    monkeypatch.setattr(m, "decode_step", lambda *a, **kw: 1 / 0)
+    with pytest.raises(ZeroDivisionError):
+        m.generate(prompt, 4)
+    assert m.training
+    draft.eval()
+    draft.generate(prompt, 2)
+    assert not draft.training
