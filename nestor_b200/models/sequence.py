@@ -217,7 +217,6 @@ def apply_recipe_variants(model: nn.Module, mup: ReferenceMupConfig) -> None:
                     adamw(mlp.layers[-1].weight, 1.0)
 
 
-@register_model(SequenceModelConfig)
 @contextlib.contextmanager
 def _evaluating(*models: nn.Module):
     """The models in evaluation mode, and as they were behind it, however it is left."""
@@ -232,6 +231,7 @@ def _evaluating(*models: nn.Module):
             m.train(training)
 
 
+@register_model(SequenceModelConfig)
 class SequenceModel(nn.Module):
     """adapter -> backbone -> head, each built from its config through the registries.
 
