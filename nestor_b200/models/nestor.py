@@ -449,6 +449,7 @@ class NestorKVCache:
             return LayerKVCache(B, s.G, max_len, s.heads, s.head_dim, device, dtype)
 
         self.blocks = [[layer(blk.spec) for _ in blk.layers] for blk in backbone.blocks]
+        self.kernels = self.eight_bit and any(c.kernels for blk in self.blocks for c in blk)
         self.columns = [blk.spec.G for blk in backbone.blocks]
         self.batch, self.max_len = B, max_len
         self._length = 0

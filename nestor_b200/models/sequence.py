@@ -17,6 +17,7 @@ import torch
 from torch import Tensor, nn
 
 from nestor_b200 import ops
+from nestor_b200.ops import _lib
 from nestor_b200.configs.model import (
     LanguageModelingHeadConfig, NestorConfig, ReferenceMupConfig, SequenceModelConfig, TextAdapterConfig,
 )
@@ -231,6 +232,13 @@ def _evaluating(*models: nn.Module):
             m.train(training)
 
 
+def _check_kernels(cache) -> None:
+    """Raise if a kernel of an 8-bit decode state has reported a failure (reads one word, so it waits for the step)."""
+
+    if getattr(cache, "kernels", False):
+        _lib.check_status(cache.positions.device)
+
+
 @register_model(SequenceModelConfig)
 class SequenceModel(nn.Module):
     """adapter -> backbone -> head, each built from its config through the registries.
@@ -421,12 +429,14 @@ class SequenceModel(nn.Module):
         logits = self._prefill(prompt, cache)
         out = [prompt]
         for i in range(max_new_tokens):
+            _check_kernels(cache)          # (before a draw from what they left, which may be NaN)
             if temperature > 0:
                 nxt = torch.multinomial(torch.softmax(logits / temperature, dim=-1), 1, generator=generator).squeeze(1)
             else:
                 nxt = logits.argmax(dim=-1)
             out.append(nxt.unsqueeze(1))
             logits = self.decode_step(nxt, cache)
+        _check_kernels(cache)
         return torch.cat(out, dim=1)
 
     def _generate_with_draft(self, prompt: Tensor, max_new_tokens: int, temperature: float, generator: torch.Generator | None,
@@ -455,6 +465,7 @@ class SequenceModel(nn.Module):
             tokens, probs, cur = [], [], last
             for i in range(n):
                 logits = draft.decode_step(cur, caches[1])
+                _check_kernels(caches[1])
                 if temperature > 0:
                     probs.append(torch.softmax(logits / temperature, dim=-1))
                     cur = torch.multinomial(probs[-1], 1, generator=generator).squeeze(1)
@@ -464,6 +475,7 @@ class SequenceModel(nn.Module):
             draft.decode_step(cur, caches[1])                                # (the last proposal enters its cache as well)
             x = torch.stack(tokens, dim=1)
             logits = self.decode_step(torch.cat((last.unsqueeze(1), x), dim=1), caches[0])
+            _check_kernels(caches[0])
             if temperature > 0:
                 target, q = torch.softmax(logits / temperature, dim=-1), torch.stack(probs, dim=1)
             else:

@@ -453,3 +453,36 @@ def test_a_refused_or_failing_generation_leaves_the_training_mode(tiny_scale, mo
     draft.eval()
     draft.generate(prompt, 2)
     assert not draft.training
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("drafted", [False, True])
+def test_generation_reports_what_its_kernels_report(drafted, tiny_scale, monkeypatch):
+    """A wait that ran out leaves NaN logits: an error before anything is drawn from them, and the device goes on."""
+
+    from nestor_b200.ops import _lib, cuda_decode
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "nestor", 8).cuda()
+    kw = dict(draft=tiny(tiny_scale, "dense", 9).cuda(), draft_tokens=3) if drafted else {}
+    prompt = torch.randint(0, 100263, (3, 9), device=DEV)
+    g = torch.Generator(DEV)
+    want = m.generate(prompt, 5, 0.7, g.manual_seed(1), torch.int8, **kw)
+    monkeypatch.setattr(cuda_decode, "WAIT_POLLS", 0)
+    with pytest.raises(RuntimeError, match="wait gave up"):
+        m.generate(prompt, 5, 0.7, g.manual_seed(1), torch.int8, **kw)
+    monkeypatch.undo()
+    assert torch.equal(want, m.generate(prompt, 5, 0.7, g.manual_seed(1), torch.int8, **kw))
+    _lib.status_word(torch.device(DEV, 0)).fill_(7)
+    with pytest.raises(RuntimeError, match="capacity"):
+        m.generate(prompt, 1, 0.0, None, torch.int8, **kw)
+    assert torch.isfinite(m.generate(prompt, 2)).all()            # an fp32 state runs no kernel that could report
+    _lib.check_status(torch.device(DEV, 0))
+
+
+def test_generation_on_the_cpu_asks_no_device(tiny_scale, monkeypatch):
+    from nestor_b200.ops import _lib
+    from test_decode_8bit import tiny
+    monkeypatch.setattr(_lib, "check_status", lambda device: 1 / 0)
+    m = tiny(tiny_scale, "dense", 5)
+    assert not m.init_kv_cache(1, 4, dtype=torch.int8).kernels
+    assert m.generate(torch.randint(0, 100263, (1, 3)), 2, cache_dtype=torch.int8).shape == (1, 5)
