@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from nestor_b200 import ops
+from nestor_b200.ops import decode as D
 from test_decode_ops import CODES, TYPES, check_attention, filled, same, to, values64
 
 DEV = "cuda"
@@ -486,3 +487,122 @@ def test_generation_on_the_cpu_asks_no_device(tiny_scale, monkeypatch):
     m = tiny(tiny_scale, "dense", 5)
     assert not m.init_kv_cache(1, 4, dtype=torch.int8).kernels
     assert m.generate(torch.randint(0, 100263, (1, 3)), 2, cache_dtype=torch.int8).shape == (1, 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("hd", [30, 40, 101])
+def test_long_appends_that_begin_inside_a_block(code, kind, hd):
+    """Pieces of a prompt: a list begins anywhere in a block and goes on over two further blocks and more. The originals
+    that were kept show when the list steps back and goes on."""
+
+    g = torch.Generator().manual_seed(hd)
+    L, H = 7, 2
+    host = ops.kv8_cache(L, H, 900, hd, "cpu", code, kind)
+    dev = to(host, DEV)
+    at = [0] * L
+    rounds = [([10, 63, 1, 64, 65, 33, 0], 0), ([130, 200, 193, 120, 191, 95, 129], 0), ([300, 1, 128, 129, 0, 160, 64], 0),
+              ([1, 2, 64, 1, 70, 3, 5], 33), ([140, 150, 1, 190, 260, 64, 130], 64), ([0] * L, 50)]
+    for i, (counts, back) in enumerate(rounds):
+        if back:
+            at = [max(0, a - back) for a in at]
+            ops.kv8_truncate(host, i32(at))
+            ops.kv8_truncate(dev, i32(at, DEV))
+            assert same(host, dev), i
+        rows = sum(counts) + 1
+        k, v = (torch.randn(rows, H, hd, generator=g).to(kind) * (1 + torch.arange(rows) % 5).view(-1, 1, 1)).to(kind), torch.randn(rows, H, hd, generator=g).to(kind)
+        for cache, d in ((host, "cpu"), (dev, DEV)):
+            ops.kv8_append(cache, k.to(d), v.to(d), seg_of(counts, d), i32(at, d), max_rows=max(1, *counts))
+        assert same(host, dev), i
+        at = [a + n for a, n in zip(at, counts)]
+    from nestor_b200.ops import _lib
+    _lib.check_status(torch.device(DEV, 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("kind,hd,group", [(torch.bfloat16, 40, 1), (torch.float32, 60, 1), (torch.float16, 80, 2)])
+def test_a_prompt_in_pieces(code, kind, hd, group):
+    """Appended and attended to in pieces, as a model feeds a prompt: many rows a list, lists that begin inside blocks."""
+
+    g = torch.Generator().manual_seed(hd)
+    L, H = 3, 2
+    cache = ops.kv8_cache(L, H, 600, hd, DEV, code, kind)
+    at = [0] * L
+    for counts in ([170, 91, 33], [150, 0, 131], [70, 193, 1]):
+        seg, rows = seg_of(counts, DEV), sum(counts)
+        k, v = (torch.randn(rows, H, hd, generator=g).to(kind).to(DEV) for _ in range(2))
+        ops.kv8_append(cache, k, v, seg, i32(at, DEV), max_rows=max(counts))
+        at = [a + n for a, n in zip(at, counts)]
+        q = (torch.randn(rows, H * group, hd, generator=g) * 2).to(kind).to(DEV)
+        got = ops.kv8_attention(q, cache, seg, i32(at, DEV), 1 / hd ** 0.5, max_rows=max(counts))
+        check_attention(q, cache, seg, at, 1 / hd ** 0.5, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hd,group", [(30, 3), (64, 1), (64, 4), (80, 2), (101, 1), (128, 8)])
+def test_attention_in_pieces_that_are_joined(code, kind, hd, group):
+    """Units and the join with every width class, one and two column tiles and several tiles a list."""
+
+    lengths, counts = [3000, 130, 700, 1], [5, 3, 1, 1]
+    cache, _, _ = filled(lengths, 2, hd, code, kind, seed=hd, capacity=8256, device=DEV)
+    g = torch.Generator().manual_seed(8)
+    q = (torch.randn(10, 2 * group, hd, generator=g) * torch.randn(10, 2 * group, 1, generator=g).exp() * 2).to(kind).to(DEV)
+    seg = seg_of(counts, DEV)
+    got = ops.kv8_attention(q, cache, seg, i32(lengths, DEV), 1 / hd ** 0.5, max_rows=5)
+    check_attention(q, cache, seg, lengths, 1 / hd ** 0.5, got)
+    assert torch.equal(got, ops.kv8_attention(q, cache, seg, i32(lengths, DEV), 1 / hd ** 0.5, max_rows=5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("code", CODES)
+def test_long_lines_of_wide_heads(code, kind):
+    """Units fetched at run time with the ring of half blocks, two column tiles, several tiles a list."""
+
+    L, H, blocks, hd, group = 24, 4, 420, 104, 4
+    cache = random_cache(L, H, blocks, hd, code, 5, kind)
+    counts, lengths = [5] * L, [blocks * 64 - 17 * l if l % 8 else 60 + l for l in range(L)]
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(5 * L, H * group, hd, generator=g).to(kind).to(DEV)
+    got = ops.kv8_attention(q, cache, seg_of(counts, DEV), i32(lengths, DEV), 0.05, max_rows=5)
+    for l in (1, 8, 23):
+        part = D.KV8Cache(*(c.view(torch.int8)[l : l + 1].view(code) for c in (cache.k_codes, cache.v_codes)),
+                          *(t[l : l + 1] for t in (cache.k_scale, cache.v_scale, cache.k_open, cache.v_open)))
+        check_attention(q[5 * l : 5 * l + 5], part, seg_of([5], DEV), [lengths[l]], 0.05, got[5 * l : 5 * l + 5])
+    assert torch.equal(got, ops.kv8_attention(q, cache, seg_of(counts, DEV), i32(lengths, DEV), 0.05, max_rows=5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("code", CODES)
+def test_the_join_of_many_items(code):
+    """More (row, head) items than 32 for each multiprocessor, lists of one to seven blocks that units cut anywhere."""
+
+    L = 400
+    lengths = [1 + (l * 61) % 440 for l in range(L)]
+    cache, _, _ = filled(lengths, 16, 24, code, torch.bfloat16, seed=3, device=DEV)
+    q = torch.randn(L, 16, 24, device=DEV).bfloat16()
+    assert L * 16 > 32 * torch.cuda.get_device_properties(0).multi_processor_count
+    seg = seg_of([1] * L, DEV)
+    got = ops.kv8_attention(q, cache, seg, i32(lengths, DEV), 0.2)
+    check_attention(q, cache, seg, lengths, 0.2, got)
+
+
+@pytest.mark.gpu
+def test_greedy_decoding_with_drafts_on_the_gpu_is_the_models_own(tiny_scale):
+    """Over an fp32 state the scoring of a round is the same single steps, so the tokens are the same."""
+
+    from test_decode_8bit import tiny
+    m, other = tiny(tiny_scale, "nestor", 3).cuda(), tiny(tiny_scale, "dense", 4).cuda()
+    near = tiny(tiny_scale, "nestor", 3).cuda()
+    torch.manual_seed(11)
+    with torch.no_grad():
+        for p in near.parameters():
+            p.add_(torch.randn_like(p) * p.abs().mean() * 0.02)
+    prompt = torch.randint(0, 100263, (3, 5), device=DEV)
+    want = m.generate(prompt, 12)
+    for draft, n in ((m, 4), (other, 1), (near, 3), (near, 6)):
+        assert torch.equal(want, m.generate(prompt, 12, draft=draft, draft_tokens=n))
