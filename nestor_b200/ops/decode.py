@@ -77,6 +77,9 @@ class KV8Cache:
         self.__dict__.update(k_codes=k_codes, v_codes=v_codes, k_scale=k_scale, v_scale=v_scale, k_open=k_open, v_open=v_open,
                              lists=L, heads=H, blocks=nb, units=U, capacity=nb * BLOCK, head_dim=D, device=device,
                              is_cuda=device.type == "cuda", dtype=code, open_dtype=kind)
+        if self.is_cuda:
+            from nestor_b200.ops import _lib
+            _lib.status_word(device)             # (made here, not by a first step that may be under graph capture)
 
     def __setattr__(self, name: str, value) -> None:
         raise AttributeError(f"the {name} of a KV8Cache is fixed (its kernels keep an argument block of it); build another one")
@@ -98,11 +101,7 @@ def kv8_cache(lists: int, heads: int, capacity: int, head_dim: int, device=None,
     codes = lambda: torch.zeros(lists, heads, nb, -(-head_dim // 8), 512, dtype=torch.uint8, device=device).view(dtype)   # noqa: E731
     scale = lambda: torch.zeros(lists, heads, nb, dtype=torch.float32, device=device)                       # noqa: E731
     held = lambda: torch.zeros(lists, heads, 2, BLOCK, head_dim, dtype=open_dtype, device=device)           # noqa: E731
-    cache = KV8Cache(codes(), codes(), scale(), scale(), held(), held())
-    if cache.is_cuda:
-        from nestor_b200.ops import _lib
-        _lib.status_word(cache.device)           # (made here, not by a first step that may be under graph capture)
-    return cache
+    return KV8Cache(codes(), codes(), scale(), scale(), held(), held())
 
 
 # ----------------------------------------------------------------------------- argument checks (both bodies)

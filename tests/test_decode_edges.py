@@ -606,3 +606,14 @@ def test_greedy_decoding_with_drafts_on_the_gpu_is_the_models_own(tiny_scale):
     want = m.generate(prompt, 12)
     for draft, n in ((m, 4), (other, 1), (near, 3), (near, 6)):
         assert torch.equal(want, m.generate(prompt, 12, draft=draft, draft_tokens=n))
+
+
+@pytest.mark.gpu
+def test_a_cache_of_given_tensors_brings_the_status_word(monkeypatch):
+    """Not its first step, which may be under capture: the word would live in that graph's memory."""
+
+    from nestor_b200.ops import _lib
+    cache = ops.kv8_cache(1, 1, 64, 8, DEV)
+    monkeypatch.setattr(_lib, "_status", {})
+    D.KV8Cache(*(getattr(cache, f) for f in ("k_codes", "v_codes", "k_scale", "v_scale", "k_open", "v_open")))
+    assert list(_lib._status) == [0]
