@@ -65,7 +65,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float x) { return __
 // layout, so nothing passes through shared memory but the warps' maxima. The values' layout is the transpose of each
 // 8 x 8 tile: their codes go through movmatrix as 16-bit numbers. Instructions, not HBM, are the bound: about 14 an
 // element, half of what a tile in shared memory took (197k rows x 3 heads x 40 in bf16: 55 us instead of 108; HBM alone
-// would take 22).
+// would take 22). Four CTAs an SM leave 64 registers a thread, of which 16-bit rows in pairs spill 12 (48 to 52 bytes).
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // softmax; a block's scales multiply its scores and its partial output in fp32.
 //
 // What bounds it: one query reads 2 bytes of cache for 4 flops, so HBM does (192 lists of 6144 to 12288 entries x 5 x 40,
-// int8, 0.71 GB: 125 us, 5.7 TB/s with both launches). The tensor pipe is used because a column tile of 8 costs no more
+// int8, 0.71 GB: 127 us, 5.6 TB/s with both launches; 143 us with a cold L2). The tensor pipe is used because a column tile of 8 costs no more
 // than one query; the conversion (0.75 instructions a code) is then the largest part of a warp's work.
 //
 // Precision. q is scaled per column by a power of two that takes its largest element into [2^14, 2^15), and rounded to
@@ -442,8 +442,12 @@ __global__ void __launch_bounds__(256) read_kernel(nb_kv8_cache c, nb_kv8_rows p
 // lines: one unit a warp, of two blocks at least. Long ones (32 blocks a warp and more): five sixths in one unit a warp,
 // the rest in as many smaller ones that the warps fetch as they finish, because equal shares end up to a quarter apart
 // (0.7 GB: the last warp at 128 us instead of 117). A unit costs some 3 us beside its blocks (queries, scales, its piece)
-// and twice the units cost the join 4 us: a line of 20 blocks a warp took 92 us so and takes 80 without, and more and
+// and twice the units cost the join 4 us: a line of 20 blocks a warp took 92 us so and takes 82 without, and more and
 // smaller units lost as well.
+//
+// Prompts. A piece of hundreds of rows a list takes a tile of 16 columns through the whole list at a time, and every tile
+// converts its codes again: 64 lists x 384 rows over 1152 entries, 3 x 40, take 165 us (69 TFLOP/s), 8 x 512 over 1536,
+// 16 x 60, 227 us (89 TFLOP/s), a twentieth of the tensor rate. Tiles of 64 rows and more would need a kernel of their own.
 constexpr float kShift = 7.f;        // log2 of the factor on the probabilities
 constexpr float kTop = 15.f;         // the same where they are relative to their block's maximum
 constexpr float kSlack = 8.f;        // how far (log2) a score may pass the running maximum; 2^(kShift + kSlack) fits fp16
@@ -571,7 +575,10 @@ __device__ __forceinline__ float tile_max(const float (&s)[4][4], int i) {
 // One CTA an SM, as many warps as its registers carry. Shared memory of one warp: a ring filled by bulk copies that the
 // warp itself issues. Nothing is shared between warps after the prologue, so there is no barrier but the copies' own.
 // Narrow heads: two stages of a block (keys and values together, one wait a block). Wide heads: three stages of half a
-// block, which leaves room for more warps. 16 x 10 KB, 16 x 12 KB, 12 x 15 KB or 8 x 24 KB.
+// block, which leaves room for more warps. 16 x 10 KB, 16 x 12 KB, 12 x 15 KB or 8 x 24 KB. Measured against the other ring,
+// with as many warps as then fit (long lists on the device, us): heads of 40 127 and 130, 5 rows x 2 heads of 40 74 and 79;
+// heads of 60 155 and 154 (12 warps), 5 rows of 60 82 and 83, 5 rows x 2 heads of 80 63 and 60, heads of 80 106 and 106 (10
+// warps), heads of 128 119 and 120 (6 warps), 8 heads of 128 on one in fp32 38 and 40 (6 warps).
 __host__ __device__ constexpr int halves_of(int umax) { return umax <= 5 ? 2 : 1; }
 __host__ __device__ constexpr int stages_of(int umax) { return umax <= 5 ? 2 : 3; }
 __host__ __device__ constexpr int warps_of(int umax, int nt) { return nt > 1 ? (umax <= 5 ? 12 : 8) : umax <= 8 ? 16 : umax <= 10 ? 12 : 8; }
@@ -1442,8 +1449,9 @@ Plan plan_of(int L, int H, int nb, int D, int rows, int max_rows, int group) {
   p.sms = multiprocessors();
   p.tasks = std::min(long(rows) * group, std::min(long(rows), long(L)) * ((columns + p.cols - 1) / p.cols)) * H;
   // by tasks: at most two a CTA and four blocks a warp (4096 entries of a narrow head); beyond that the longest task would
-  // decide. 80 lists x 3 heads of 2000 entries take 16.7 us instead of 18.5, 8 x 2 of 400 7.1 instead of 8.8, and a call
-  // costs the host 19 us instead of 23 (one launch, no workspace).
+  // decide. 8 lists x 2 heads of 400 entries take 7.4 us instead of 11.2 with units, and a call costs the host 19 us instead
+  // of 23 (one launch, no workspace). Towards the rule's end the device gains nothing (80 x 3 x 40 of 2000 entries: 17.5 and
+  // 17.4; 80 x 3 x 60 of 2250: 24.5 instead of 21.9), the host's call still does.
   p.by_task = L <= kMaxLists && nb <= 4 * p.warps && p.tasks <= 2l * p.sms;
   p.bytes = p.by_task ? 0 : 16 + 8l * rows * H * group + long(p.sms) * p.warps * (1 + kShares) * 2 * slot_floats(U, p.cols) * 4;
   return p;

@@ -332,10 +332,13 @@ def kv8_attention(q: Tensor, cache: KV8Cache, seg_start: Tensor, lengths: Tensor
     ``q [rows, Hq, head_dim]`` (bf16, fp16 or fp32; ``Hq`` a multiple of the cache's heads, query head ``h`` reads key
     head ``h * H // Hq``). ``lengths [L]`` counts the entries of each list with the new rows' own among them, so row
     ``a`` of the ``n`` rows of list ``l`` sees the first ``lengths[l] - (n - 1 - a)`` entries. Softmax of
-    ``scale * q . k`` in fp32, output in ``q.dtype``; a row that sees nothing gives zeros. Rows behind ``seg_start[-1]``
+    ``scale * q . k`` with fp32 sums, output in ``q.dtype``; a row that sees nothing gives zeros. (The kernel's products take
+    fp16 numbers: one for a 16-bit query element, two, 22 bits, for an fp32 one; one for a weight whose output is bf16, 11
+    bits and no less than 2^-32 of the row's largest, two for the others.) Rows behind ``seg_start[-1]``
     are left as they are in ``out`` (which may be ``q`` itself, but must not overlap it otherwise) and are zeros without
     it. ``max_rows`` (how many rows a list brings at most) only steers speed. ``lengths`` beyond the capacity count as the
-    capacity and are reported like in :func:`kv8_append`.
+    capacity and are reported like in :func:`kv8_append`, and so are bounds that do not ascend from 0; rows that no list with
+    valid bounds covers are zeros. Rows whose codes a kernel waited for in vain are NaN, and reported.
     """
 
     check_attention(q, cache, seg_start, lengths, scale, max_rows, out)
