@@ -1020,7 +1020,7 @@ class Nestor(Backbone):
                              f"{', or the same number to each' if cache.eight_bit else ''}; got {x0.shape[0]} rows")
         if cache.eight_bit and cache.length + S > cache.max_len:
             raise ValueError(f"key/value cache of {cache.max_len} positions per column is full")
-        with ops.oracle_ops():        # per-token work: the PyTorch statement of the ops on any device
+        with ops.kernel_ops(False):   # per-token work: the PyTorch statement of the ops on any device, in this thread
             narrow, wide, x, aux = [x0], [x0], x0, []
             for i, (block, bcache) in enumerate(zip(self.blocks, cache.blocks)):
                 exports, x, a = block(x, list(wide) if self.wide_reads else narrow, B, S, cd, pos, self.column_mode, None,

@@ -617,3 +617,23 @@ def test_a_cache_of_given_tensors_brings_the_status_word(monkeypatch):
     monkeypatch.setattr(_lib, "_status", {})
     D.KV8Cache(*(getattr(cache, f) for f in ("k_codes", "v_codes", "k_scale", "v_scale", "k_open", "v_open")))
     assert list(_lib._status) == [0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.int8])
+def test_a_decode_step_leaves_other_threads_ops_alone(dtype, tiny_scale, monkeypatch):
+    import threading
+    from nestor_b200.models.nestor import Layer
+    from test_decode_8bit import tiny
+    m = tiny(tiny_scale, "nestor", 5)
+    seen, step = [], Layer.attention_step
+
+    def look(self, *args):
+        t = threading.Thread(target=lambda: seen.append(ops.use_kernels(OnDevice)))
+        t.start()
+        t.join()
+        seen.append(ops.use_kernels(OnDevice))
+        return step(self, *args)
+
+    monkeypatch.setattr(Layer, "attention_step", look)
+    m.decode_step(torch.randint(0, 100263, (2,)), m.init_kv_cache(2, 4, dtype=dtype))
+    assert seen and all(seen[::2]) and not any(seen[1::2])
